@@ -32,9 +32,11 @@ CSRC = PKG / "csrc"
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 ARCH = os.environ.get("FCMOE_OFFLOAD_ARCH", "gfx950")
 
-HIP_SOURCES = ["fcmoe_api.hip", "fcmoe_route.hip", "fcmoe_quant.hip", "fcmoe_gemm.hip", "fcmoe_gemm_lds.hip", "fcmoe_gemm_smallm.hip", "fcmoe_gemm_mid.hip", "fcmoe_combine.hip", "fcmoe_decode_tail.hip", "fcmoe_decode_bf16.hip", "fcmoe_router.hip"]
+HIP_SOURCES = ["fcmoe_api.hip", "fcmoe_route.hip", "fcmoe_quant.hip", "fcmoe_gemm.hip", "fcmoe_gemm_lds.hip", "fcmoe_gemm_smallm.hip", "fcmoe_gemm_mid.hip", "fcmoe_combine.hip", "fcmoe_decode_tail.hip", "fcmoe_decode_bf16.hip", "fcmoe_router.hip", "fcmoe_latent_rows.hip",
+               "fcmoe_head_project.hip", "fcmoe_absorbed.hip", "fcmoe_expanded.hip"]
 # bench-only measurement probes: a library of their own (fcmoe_probe.h), linked against libfcmoe.so
 PROBE_SOURCES = ["fcmoe_probe.hip"]
+EXT_SOURCES = ["moe_ext.cpp", "latent_ext.cpp"]
 HIP_FLAGS = [
     f"--offload-arch={ARCH}",
     "-O3",
@@ -119,11 +121,10 @@ def build_ext() -> Path:
     torch_lib = Path(torch.__file__).resolve().parent / "lib"
     incs = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], str(ROCM / "include")]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = [
-        os.environ.get("CXX", "g++"),
+    cxx = os.environ.get("CXX", "g++")
+    flags = [
         "-O2",
         "-fPIC",
-        "-shared",
         "-std=c++17",
         "-D__HIP_PLATFORM_AMD__=1",
         "-DUSE_ROCM=1",
@@ -131,7 +132,20 @@ def build_ext() -> Path:
         "-DTORCH_API_INCLUDE_EXTENSION_H",
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
         *[f"-I{i}" for i in incs],
-        str(CSRC / "moe_ext.cpp"),
+    ]
+    BUILD_DIR.mkdir(parents=True, exist_ok=True)
+
+    def compile_one(src: str) -> str:
+        obj = str(BUILD_DIR / (src + ".o"))
+        _run([cxx, *flags, "-c", str(CSRC / src), "-o", obj])
+        return obj
+
+    with ThreadPoolExecutor(max_workers=len(EXT_SOURCES)) as ex:
+        objs = list(ex.map(compile_one, EXT_SOURCES))
+    cmd = [
+        cxx,
+        "-shared",
+        *objs,
         "-o",
         str(EXT) + ".tmp",
         f"-L{torch_lib}",

@@ -59,6 +59,84 @@ class MoeArgs(ctypes.Structure):
     ]
 
 
+class HeadNormRopeArgs(ctypes.Structure):
+    """Mirror of ``struct fcmoe_head_norm_rope_args``."""
+
+    _fields_ = [
+        ("x", _P), ("tokens", _I64), ("heads", _I64), ("dim", _I64),
+        ("x_token_stride", _I64), ("x_head_stride", _I64),
+        ("positions", _P), ("positions_i64", _I),
+        ("cos_sin", _P), ("table_rows", _I64), ("rope_dim", _I64),
+        ("weight", _P), ("eps", ctypes.c_float),
+        ("normalize", _I), ("inverse", _I), ("interleaved", _I),
+        ("out", _P), ("out_token_stride", _I64), ("out_head_stride", _I64),
+    ]
+
+
+class LatentCacheDesc(ctypes.Structure):
+    """Mirror of ``struct fcmoe_latent_cache``."""
+
+    _fields_ = [
+        ("latent", _P), ("rope", _P), ("scale", _P),
+        ("pages", _I64), ("page_size", _I64), ("latent_dim", _I64), ("rope_dim", _I64),
+        ("latent_page_stride", _I64), ("latent_row_stride", _I64),
+        ("rope_page_stride", _I64), ("rope_row_stride", _I64),
+        ("scale_page_stride", _I64), ("e4m3", _I),
+    ]
+
+
+class LatentAppendArgs(ctypes.Structure):
+    """Mirror of ``struct fcmoe_latent_append_args``."""
+
+    _fields_ = [
+        ("kv", _P), ("tokens", _I64), ("kv_row_stride", _I64),
+        ("positions", _P), ("slots", _P), ("positions_i64", _I), ("slots_i64", _I),
+        ("cos_sin", _P), ("table_rows", _I64), ("rot_dim", _I64),
+        ("weight", _P), ("eps", ctypes.c_float), ("interleaved", _I),
+        ("rows_out", _P), ("cache", LatentCacheDesc),
+    ]
+
+
+class HeadProjectionArgs(ctypes.Structure):
+    """Mirror of ``struct fcmoe_head_projection_args``."""
+
+    _fields_ = [
+        ("x", _P), ("tokens", _I64), ("heads", _I64), ("n", _I64), ("k", _I64),
+        ("x_token_stride", _I64), ("x_head_stride", _I64),
+        ("w_packed", _P), ("out", _P), ("out_token_stride", _I64), ("out_head_stride", _I64),
+    ]
+
+
+class AbsorbedArgs(ctypes.Structure):
+    """Mirror of ``struct fcmoe_absorbed_args``."""
+
+    _fields_ = [
+        ("q_latent", _P), ("q_rope", _P), ("tokens", _I64), ("heads", _I64), ("batch", _I64),
+        ("q_latent_token_stride", _I64), ("q_latent_head_stride", _I64),
+        ("q_rope_token_stride", _I64), ("q_rope_head_stride", _I64),
+        ("cache", LatentCacheDesc),
+        ("page_table", _P), ("table_width", _I64), ("page_table_stride", _I64),
+        ("kv_lens", _P), ("query_starts", _P), ("scale", ctypes.c_float),
+        ("out", _P), ("out_token_stride", _I64), ("out_head_stride", _I64),
+        ("lse", _P), ("zero_uncovered", _I), ("workspace", _P), ("workspace_bytes", _SZ),
+    ]
+
+
+class ExpandedArgs(ctypes.Structure):
+    """Mirror of ``struct fcmoe_expanded_args``."""
+
+    _fields_ = [
+        ("q", _P), ("kv", _P), ("k_rope", _P),
+        ("tokens", _I64), ("keys", _I64), ("heads", _I64), ("batch", _I64),
+        ("nope_dim", _I64), ("rope_dim", _I64), ("v_dim", _I64),
+        ("q_token_stride", _I64), ("q_head_stride", _I64),
+        ("kv_token_stride", _I64), ("kv_head_stride", _I64), ("k_rope_token_stride", _I64),
+        ("query_starts", _P), ("kv_starts", _P), ("scale", ctypes.c_float), ("causal", _I),
+        ("out", _P), ("out_token_stride", _I64), ("out_head_stride", _I64),
+        ("lse", _P), ("zero_uncovered", _I), ("workspace", _P), ("workspace_bytes", _SZ),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/fcmoe.h.
 SIGNATURES = {
     "fcmoe_last_error": (ctypes.c_char_p, []),
@@ -88,6 +166,13 @@ SIGNATURES = {
     "fcmoe_stage_timing_enable": (_I, [_I]),
     "fcmoe_stage_timing_read": (_I, [_P, _P]),
     "fcmoe_w8a8_prefill_plan": (_I, [_P, _P]),
+    "fcmoe_head_norm_rope": (_I, [ctypes.POINTER(HeadNormRopeArgs), _P]),
+    "fcmoe_latent_cache_append": (_I, [ctypes.POINTER(LatentAppendArgs), _P]),
+    "fcmoe_head_projection": (_I, [ctypes.POINTER(HeadProjectionArgs), _P]),
+    "fcmoe_absorbed_attention_workspace_bytes": (_SZ, [ctypes.POINTER(AbsorbedArgs)]),
+    "fcmoe_absorbed_attention": (_I, [ctypes.POINTER(AbsorbedArgs), _P]),
+    "fcmoe_expanded_attention_workspace_bytes": (_SZ, [ctypes.POINTER(ExpandedArgs)]),
+    "fcmoe_expanded_attention": (_I, [ctypes.POINTER(ExpandedArgs), _P]),
 }
 
 FCMOE_STAGE_COUNT = 24

@@ -373,4 +373,7 @@ struct SmallBatchArgs {
 };
 int small_batch_bf16_launch(const SmallBatchArgs& a, bool w8, bool tail, hipStream_t stream);
 
+// ---- latent attention (fcmoe_latent_rows.hip) ----
+int check_latent_cache(const fcmoe_latent_cache& c, const char* what);
+
 }  // namespace fcmoe

@@ -603,6 +603,8 @@ std::vector<std::string> available_backends() { return {kBackendName}; }
 
 }  // namespace
 
+void bind_latent_attention(pybind11::module_& m);  // latent_ext.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "MI355X (gfx950) fused MoE host extension over libfcmoe";
   m.def("available_backends", &available_backends);
@@ -620,4 +622,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("i8gemm_prepare", &i8gemm_prepare);
   m.def("i8gemm_dynamic_scaled_mm", &i8gemm_dynamic_scaled_mm);
   m.def("i8gemm_dynamic_scaled_mm_pair", &i8gemm_dynamic_scaled_mm_pair);
+  bind_latent_attention(m);
 }

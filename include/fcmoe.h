@@ -203,6 +203,156 @@ int fcmoe_i8gemm_pair(const uint16_t* x, int64_t m, int64_t k, const void* w1_pa
                       int64_t n1, const void* w2_packed, const float* w2_scale, int64_t n2, uint16_t* out1,
                       uint16_t* out2, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
+/* ---- latent attention ---------------------------------------------------
+ *
+ * The steps between the W8A8 projections of a DeepSeek latent-attention layer:
+ * what the reference's adapter leaves to its caller's attention backend. No
+ * counterpart in the fused-MoE reference path. All tensors are bf16 unless
+ * stated; strides are in elements, the last dimension is contiguous. */
+
+/* Per-head RMS norm and position rotation of x [tokens, heads, dim], one pass:
+ * y = x * rsqrt(mean(x^2) + eps) * weight (normalize != 0; weight optional),
+ * then the last rope_dim values of each head are rotated by the angles of
+ * table row positions[token]: cos_sin [table_rows, rope_dim] fp32, cosines of
+ * the rope_dim / 2 pairs, then their sines. interleaved: pairs are
+ * neighbours; else rope_dim / 2 apart. inverse: by the negative angles. A
+ * position outside the table makes the rotated values NaN. out may be x. */
+typedef struct fcmoe_head_norm_rope_args {
+  const uint16_t* x;
+  int64_t tokens, heads, dim;
+  int64_t x_token_stride, x_head_stride;
+  const void* positions; /* [tokens] int32, or int64 if positions_i64 */
+  int positions_i64;
+  const float* cos_sin;
+  int64_t table_rows, rope_dim;
+  const uint16_t* weight; /* [dim] or NULL */
+  float eps;
+  int normalize, inverse, interleaved;
+  uint16_t* out;
+  int64_t out_token_stride, out_head_stride;
+} fcmoe_head_norm_rope_args;
+int fcmoe_head_norm_rope(const fcmoe_head_norm_rope_args* args, hipStream_t stream);
+
+/* A paged cache of latent rows: token slot s lies in page s / page_size at row
+ * s % page_size. latent [pages, page_size, latent_dim] and rope [pages,
+ * page_size, rope_dim] are bf16, or (e4m3 != 0) OCP e4m3 bytes that stand for
+ * byte * scale[page, row], one fp32 scale a token. Rows start at multiples of
+ * 16 bytes. latent_dim 256 or 512; rope_dim 64, or 0 (rope NULL: the whole key
+ * is the latent row). */
+typedef struct fcmoe_latent_cache {
+  void* latent;
+  void* rope;
+  float* scale;
+  int64_t pages, page_size, latent_dim, rope_dim;
+  int64_t latent_page_stride, latent_row_stride;
+  int64_t rope_page_stride, rope_row_stride;
+  int64_t scale_page_stride;
+  int e4m3;
+} fcmoe_latent_cache;
+
+/* Writes rows kv [tokens, latent_dim + rope_dim] into the cache at slots
+ * [tokens]: the first latent_dim values RMS-normalised (times weight), the
+ * last rot_dim values rotated as above (rot_dim = rope_dim, or with rope_dim 0
+ * a multiple of 16 of the latent's last values). An e4m3 row's scale is
+ * max|row| / 448 (1 for a zero row). A token whose slot lies outside the cache
+ * (-1: padding) is not written. Slots of one call must differ: a slot given
+ * twice ends up with either row or a mixture. rows_out (optional): [tokens,
+ * latent_dim + rope_dim] bf16, the rows before quantisation, for every token. */
+typedef struct fcmoe_latent_append_args {
+  const uint16_t* kv;
+  int64_t tokens, kv_row_stride;
+  const void* positions;
+  const void* slots;
+  int positions_i64, slots_i64;
+  const float* cos_sin;
+  int64_t table_rows, rot_dim;
+  const uint16_t* weight;
+  float eps;
+  int interleaved;
+  uint16_t* rows_out;
+  fcmoe_latent_cache cache;
+} fcmoe_latent_append_args;
+int fcmoe_latent_cache_append(const fcmoe_latent_append_args* args, hipStream_t stream);
+
+/* out[t, h, :] = w[h] x[t, h, :]: w [heads, n, k] packed by
+ * fcmoe_pack_experts(w, 2, heads, n, k, 1, ...). n and k multiples of 8; x rows
+ * at multiples of 16 bytes, out rows of 8. fp32 accumulation. */
+typedef struct fcmoe_head_projection_args {
+  const uint16_t* x;
+  int64_t tokens, heads, n, k;
+  int64_t x_token_stride, x_head_stride;
+  const void* w_packed;
+  uint16_t* out;
+  int64_t out_token_stride, out_head_stride;
+} fcmoe_head_projection_args;
+int fcmoe_head_projection(const fcmoe_head_projection_args* args, hipStream_t stream);
+
+/* Latent attention, absorbed form, over a paged cache: query token i of the n
+ * of sequence b (query_starts[b] .. [b + 1]; NULL: one token a sequence) sees
+ * the first kv_lens[b] - n + i + 1 cached tokens,
+ *   s_j = scale * (q_latent . c_j + q_rope . r_j),  out = sum_j softmax(s)_j c_j,
+ * where page page_table[b, j / page_size] holds token j. out [tokens, heads,
+ * latent_dim]; lse [tokens, heads] fp32 (optional): log sum_j exp(s_j). A row
+ * that sees no token is 0 with lse -inf. Lengths past the page table's reach
+ * are cut to it. A page id outside the cache that a length reaches makes the
+ * sequence's rows NaN. Rows past a length may hold anything; a cached token
+ * that some query of a sequence sees has to be finite for the others too.
+ * zero_uncovered: tokens that no sequence holds become 0 (else they are left).
+ * Workspace: the partial results of key ranges that several workgroups share;
+ * its size depends on the current device's CU count. */
+typedef struct fcmoe_absorbed_args {
+  const uint16_t* q_latent; /* [tokens, heads, latent_dim] */
+  const uint16_t* q_rope;   /* [tokens, heads, rope_dim]; NULL with rope_dim 0 */
+  int64_t tokens, heads, batch;
+  int64_t q_latent_token_stride, q_latent_head_stride;
+  int64_t q_rope_token_stride, q_rope_head_stride;
+  fcmoe_latent_cache cache;
+  const int32_t* page_table; /* [batch, table_width], rows page_table_stride apart */
+  int64_t table_width, page_table_stride;
+  const int32_t* kv_lens;      /* [batch] */
+  const int32_t* query_starts; /* [batch + 1] or NULL */
+  float scale;
+  uint16_t* out;
+  int64_t out_token_stride, out_head_stride;
+  float* lse;
+  int zero_uncovered;
+  void* workspace;
+  size_t workspace_bytes;
+} fcmoe_absorbed_args;
+size_t fcmoe_absorbed_attention_workspace_bytes(const fcmoe_absorbed_args* args);
+int fcmoe_absorbed_attention(const fcmoe_absorbed_args* args, hipStream_t stream);
+
+/* Latent attention, expanded form: per-head keys and values kv [keys, heads,
+ * nope_dim + v_dim] (keys, then values) and the key part k_rope [keys,
+ * rope_dim] that the heads share; q [tokens, heads, nope_dim + rope_dim].
+ * Sequence b has query tokens query_starts[b] .. [b + 1] and keys
+ * kv_starts[b] .. [b + 1]; with causal != 0 query i of n sees the first
+ * len - n + i + 1 keys. nope_dim = v_dim = 128 or 64, rope_dim 64 or 0 (k_rope
+ * NULL). out [tokens, heads, v_dim], lse and zero_uncovered as above; keys
+ * that some query of a sequence sees have to be finite. */
+typedef struct fcmoe_expanded_args {
+  const uint16_t* q;
+  const uint16_t* kv;
+  const uint16_t* k_rope;
+  int64_t tokens, keys, heads, batch;
+  int64_t nope_dim, rope_dim, v_dim;
+  int64_t q_token_stride, q_head_stride;
+  int64_t kv_token_stride, kv_head_stride;
+  int64_t k_rope_token_stride;
+  const int32_t* query_starts;
+  const int32_t* kv_starts;
+  float scale;
+  int causal;
+  uint16_t* out;
+  int64_t out_token_stride, out_head_stride;
+  float* lse;
+  int zero_uncovered;
+  void* workspace;
+  size_t workspace_bytes;
+} fcmoe_expanded_args;
+size_t fcmoe_expanded_attention_workspace_bytes(const fcmoe_expanded_args* args);
+int fcmoe_expanded_attention(const fcmoe_expanded_args* args, hipStream_t stream);
+
 /* ---- diagnostics (stage-level parity checks) ---------------------------- */
 
 /* Grouped int8 GEMM returning raw int32 accumulators: for each expert e and
