@@ -20,6 +20,8 @@
 // Products are S^T = K Q^T and O^T = V^T P^T (fcmoe_latent.h). V = c: one LDS
 // copy of a tile serves both, read along d for S^T and through transposing
 // reads along the keys for O^T.
+#include <type_traits>
+
 #include "fcmoe_internal.h"
 #include "fcmoe_latent.h"
 
@@ -28,6 +30,16 @@ namespace fcmoe {
 namespace {
 
 constexpr int kAbsKeys = 64;  // keys of a tile
+constexpr int kBufWord3 = 0x00020000;  // raw buffer resource word 3 for gfx9: 32-bit data format, no swizzle
+
+// A row group whose tiles end up with several shares: left by the share that
+// has its first tile for the launch that joins the partial results.
+struct Joint {
+  int64_t q0;
+  int rows, row0;  // of the sequence; first of the group
+  int last;        // share with the group's last tile
+  int valid;
+};
 
 struct Absorbed {
   const uint16_t* ql;
@@ -47,7 +59,9 @@ struct Absorbed {
   float* lse;
   float* part_o;    // [2 * shares slots][rows * R]
   float* part_lse;  // [2 * shares slots][rows], base 2
+  Joint* joints;    // [shares]
   int shares;
+  int page_shift;  // log2 of a page size that is a power of two, else -1
   int zero_tail;
 };
 
@@ -77,19 +91,11 @@ __device__ __forceinline__ int absorbed_limit(const SeqSpan& s, int i) {
   return v < 0 ? 0 : v > s.len ? s.len : v;
 }
 
-// Units of the batch (every lane of a wave takes part).
-__device__ __forceinline__ int64_t total_units(const Absorbed& p, int rows) {
-  int64_t sum = 0;
-  for (int b = (int)threadIdx.x % kWave; b < p.batch; b += kWave) {
-    const SeqSpan s = absorbed_span(p, b);
-    sum += (int64_t)row_groups(p, s, rows) * key_tiles(s);
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-  return sum;
-}
-
 __device__ __forceinline__ int64_t share_begin(int64_t units, int64_t g, int64_t wgs) { return units * g / wgs; }
+__device__ __forceinline__ int share_size(int64_t units, int64_t g, int64_t wgs) {
+  const int64_t n = share_begin(units, g + 1, wgs) - share_begin(units, g, wgs);
+  return n < INT32_MAX ? (int)n : INT32_MAX;
+}
 // The workgroup whose share holds unit u.
 __device__ __forceinline__ int64_t share_of(int64_t units, int64_t u, int64_t wgs) {
   return ((u + 1) * wgs + units - 1) / units - 1;
@@ -99,36 +105,24 @@ __device__ __forceinline__ int64_t share_of(int64_t units, int64_t u, int64_t wg
 struct Segment {
   SeqSpan seq;
   int b;
-  int64_t row0;         // first row of the group
-  int t_begin, t_end;   // tiles
-  bool whole;           // all tiles of the group
-  int64_t slot;         // partial slot otherwise
+  int row0;            // first row of the group
+  int t_begin, t_end;  // tiles
+  int tiles;           // of the group
 };
 
-// The segment that starts at unit u of workgroup g's share [u, u1).
-__device__ __forceinline__ Segment next_segment(const Absorbed& p, int rows, int64_t u, int64_t u1, int64_t g) {
+// The segment that starts at unit u, `left` units before the end of its share.
+__device__ __forceinline__ Segment next_segment(const Absorbed& p, int rows, int64_t u, int left) {
   Segment s;
   int64_t before;
   s.b = find_sequence(
-      p.batch, u,
-      [&](int b) {
-        const SeqSpan q = absorbed_span(p, b);
-        return (int64_t)row_groups(p, q, rows) * key_tiles(q);
-      },
-      &before);
-  s.b = __builtin_amdgcn_readfirstlane(s.b);
-  s.seq = absorbed_span(p, s.b);
-  const int tiles = key_tiles(s.seq);
-  const int64_t rel = u - before;
-  const int64_t group = rel / tiles;
-  s.t_begin = __builtin_amdgcn_readfirstlane((int)(rel - group * tiles));
-  const int64_t end = before + (group + 1) * tiles;
-  s.t_end = __builtin_amdgcn_readfirstlane(s.t_begin + (int)((end < u1 ? end : u1) - u));
-  s.row0 = (int64_t)__builtin_amdgcn_readfirstlane((int)(group * rows));
-  s.whole = s.t_begin == 0 && s.t_end == tiles;
-  // of a share's segments only the first can start inside a group's tiles and
-  // only the last can end inside them: two slots a workgroup
-  s.slot = 2 * g + (s.t_begin == 0 ? 1 : 0);
+      p.batch, u, [&](int b) { return absorbed_span(p, b); },
+      [&](const SeqSpan& q) { return (int64_t)row_groups(p, q, rows) * key_tiles(q); }, &s.seq, &before);
+  s.tiles = key_tiles(s.seq);
+  const uint32_t rel = (uint32_t)(u - before);  // a sequence's units: its row groups times its tiles
+  const uint32_t group = rel / (uint32_t)s.tiles;
+  s.t_begin = uniform((int)(rel - group * (uint32_t)s.tiles));
+  s.t_end = uniform(s.t_begin + min(s.tiles - s.t_begin, left));
+  s.row0 = uniform((int)group * rows);
   return s;
 }
 
@@ -153,93 +147,104 @@ struct Tile {
   static constexpr int ROPE = kAbsKeys * LROW;            // key-part rows follow the latent rows
   static constexpr int BYTES = ROPE + kAbsKeys * RROW;
   static constexpr int UNITS = LROW / 16, RUNITS = P > 0 ? RROW / 16 : 1;
-  static constexpr int LLOADS = 16 * LROW / 1024;         // 1 KB loads of a wave's 16 keys
-  static constexpr int RLOADS = 16 * RROW / 1024;
+  static constexpr int RLOADS = 16 * RROW / 1024;         // 1 KB pieces of a wave's 16 key parts
 };
 
-// A value the compiler cannot see through: what depends on it is formed after this point.
-__device__ __forceinline__ int opaque(int v) {
-  asm volatile("" : "+v"(v));
-  return v;
-}
-
-// Lane l's value, in scalar registers (l the same for the whole wave).
-__device__ __forceinline__ uint64_t lane_value(uint64_t v, int l) {
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l);
-  return ((uint64_t)hi << 32) | lo;
-}
+typedef __attribute__((address_space(3))) float lds_f32;
+typedef __attribute__((address_space(3))) int lds_i32;
+typedef __attribute__((address_space(1))) v4i global_v4i;  // an address from integers is a generic one otherwise
 
 // Brings a wave's 16 keys of a tile into LDS. Lane l knows the cached row of
 // the wave's key l % 16: its page id is read one tile ahead (fetch), so that
 // the rows' addresses are there when the buffer is free.
+//
+// Latent rows go from memory straight to LDS, one load a key with its address
+// in scalar registers; they are buffer loads, because after a global load to
+// LDS the compiler waits for all of a wave's LDS reads wherever it needs one.
+// The key parts and scales (rows too short for a load each) pass through
+// registers.
 template <int R, int P, bool F8>
 struct Stager {
   using T = Tile<R, P, F8>;
   const int32_t* table;
-  int lane, wave, key_in, last_key;  // key_in: the lane's key of a tile; last_key: of the sequence
-  int page_size;
+  int wave, last_key;  // last_key: of the sequence
   int32_t id;
   int in;
-  bool bad;
+  uint64_t lat;  // the tile being brought in
+  v4i part[P > 0 ? T::RLOADS : 1];
+  float scale;
 
-  __device__ __forceinline__ void begin(const Absorbed& p, const SeqSpan& s, int b) {
-    lane = (int)threadIdx.x % kWave;
-    wave = (int)threadIdx.x / kWave;
-    key_in = 16 * wave + lane % 16;
+  __device__ __forceinline__ void begin(const Absorbed& p, const SeqSpan& s, int b, int w) {
+    wave = w;
     table = p.table + (int64_t)b * p.table_stride;
-    page_size = (int)p.c.page_size;
     last_key = s.len - 1;
-    bad = false;
   }
-  __device__ __forceinline__ void fetch(int tile) {
-    int key = tile * kAbsKeys + key_in;
+  __device__ __forceinline__ void fetch(const Absorbed& p, int tile) {
+    int key = tile * kAbsKeys + 16 * wave + lane_now() % 16;
     key = key < last_key ? key : last_key;  // keys past the length re-read its last one; their scores are masked
-    const int page = (int)((uint32_t)key / (uint32_t)page_size);
-    in = key - page * page_size;
+    const uint32_t size = (uint32_t)p.c.page_size;
+    const uint32_t page = p.page_shift >= 0 ? (uint32_t)key >> p.page_shift : (uint32_t)key / (uint32_t)opaque_uniform((int)size);
+    in = key - (int)(page * size);
     id = table[page];
   }
-  // scl: LDS, 64 scales of the buffer (8-bit rows).
-  __device__ __forceinline__ void issue(const Absorbed& p, lds_u8* dst, lds_u8* scl) {
-    int64_t page = id;
-    if ((uint64_t)page >= (uint64_t)p.c.pages) {
-      page = 0;
-      bad = true;
-    }
-    const char* lat = (const char*)p.c.latent + (page * p.c.latent_page_stride + in * p.c.latent_row_stride) * T::ELEM;
-    // Lane-dependent parts are formed here, load by load: kept across the tile
-    // loop, or all at once, they would take the registers that Q and O need.
-    const int ln = opaque(lane);
-#pragma unroll
-    for (int u = 0; u < T::LLOADS; ++u) {
-      lds_u8* to = dst + wave * (16 * T::LROW) + u * 1024;
-      if constexpr (T::UNITS == 64) {  // one key a load: its address is the same for the whole wave
-        load_lds16((const char*)lane_value((uint64_t)lat, u) + ((ln * 16) ^ (swz_key<F8>(u) * 16)), to);
-      } else {
-        constexpr int LKEYS = 1024 / T::LROW;
-        const int k = u * LKEYS + ln / T::UNITS;
-        load_lds16((const char*)__shfl((long long)lat, k) + ((ln % T::UNITS) ^ swz_key<F8>(k)) * 16, to);
-      }
-      if (u % 2 == 1) __builtin_amdgcn_sched_barrier(0);
-    }
+  // The fetched tile's latent addresses.
+  __device__ __forceinline__ void start(const Absorbed& p, lds_u8* bad_flag) {
+    const bool bad = (uint64_t)(int64_t)id >= (uint64_t)p.c.pages;
+    if (bad) id = 0;
+    if (__any(bad)) *(lds_i32*)bad_flag = 1;  // every lane writes the same
+    lat = (uint64_t)p.c.latent + (id * p.c.latent_page_stride + in * p.c.latent_row_stride) * T::ELEM;
+  }
+  // Its key parts and scales on their way to registers.
+  __device__ __forceinline__ void parts(const Absorbed& p) {
     if constexpr (P > 0) {
-      const char* rope = (const char*)p.c.rope + (page * p.c.rope_page_stride + in * p.c.rope_row_stride) * T::ELEM;
-      constexpr int RKEYS = 1024 / T::RROW;
+      const uint32_t ln = (uint32_t)lane_now();
+      const uint64_t rope = (uint64_t)p.c.rope + (id * p.c.rope_page_stride + in * p.c.rope_row_stride) * T::ELEM;
+#pragma unroll
+      for (int u = 0; u < T::RLOADS; ++u)
+        part[u] = *(const global_v4i*)(__shfl((unsigned long long)rope, u * (64 / T::RUNITS) + (int)(ln / T::RUNITS)) +
+                                       (ln % T::RUNITS) * 16);
+    }
+    if constexpr (F8) scale = p.c.scale[id * p.c.scale_page_stride + in];
+  }
+  // The latent row of key u (0 .. 15) to its place in buffer `dst`.
+  __device__ __forceinline__ void load(lds_u8* dst, int u) const {
+    const uint32_t ln = (uint32_t)lane_now();
+    const __amdgpu_buffer_rsrc_t row = __builtin_amdgcn_make_buffer_rsrc((void*)lane_value(lat, u), (short)0, T::LROW, kBufWord3);
+    if (T::UNITS == 64 || ln < T::UNITS)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(row, (__attribute__((address_space(3))) void*)(dst + (16 * wave + u) * T::LROW), 16,
+                                               (ln ^ (uint32_t)swz_key<F8>(u)) * 16, 0, 0, 0);
+  }
+  __device__ __forceinline__ void load_all(lds_u8* dst) const {
+#pragma unroll
+    for (int u = 0; u < 16; ++u) load(dst, u);
+  }
+  // The key parts and scales from registers to buffer `dst` (scales to `scl`).
+  __device__ __forceinline__ void finish(lds_u8* dst, lds_u8* scl) const {
+    const uint32_t ln = (uint32_t)lane_now();
+    if constexpr (P > 0) {
 #pragma unroll
       for (int u = 0; u < T::RLOADS; ++u) {
-        const int k = u * RKEYS + ln / T::RUNITS;
-        load_lds16((const char*)__shfl((long long)rope, k) + ((ln % T::RUNITS) ^ swz_rope<F8>(k)) * 16,
-                   dst + T::ROPE + wave * (16 * T::RROW) + u * 1024);
+        const uint32_t k = u * (64 / T::RUNITS) + ln / T::RUNITS;
+        *(__attribute__((address_space(3))) v4i*)(dst + T::ROPE + (16 * wave + k) * T::RROW +
+                                                  ((ln % T::RUNITS) ^ (uint32_t)swz_rope<F8>(k)) * 16) = part[u];
       }
     }
     if constexpr (F8) {
-      const float* s = p.c.scale + page * p.c.scale_page_stride + in;
-      if (lane < 16)
-        __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)s,
-                                         (__attribute__((address_space(3))) void*)(scl + wave * 64), 4, 0, 0);
+      if (ln < 16) *(lds_f32*)(scl + (16 * wave + ln) * 4) = scale;
     }
   }
 };
+
+// f(integral_constant<int, i>) for an i that unrolling makes known.
+template <int N, typename F>
+__device__ __forceinline__ void unroll_at(int i, F f) {
+  if constexpr (N > 0) {
+    if (i == N - 1)
+      f(std::integral_constant<int, N - 1>{});
+    else
+      unroll_at<N - 1>(i, f);
+  }
+}
 
 __device__ __forceinline__ v8bf lds_v8bf(const lds_u8* p) { return *(const __attribute__((address_space(3))) v8bf*)p; }
 __device__ __forceinline__ v4i lds_v4i(const lds_u8* p) { return *(const __attribute__((address_space(3))) v4i*)p; }
@@ -247,100 +252,231 @@ __device__ __forceinline__ v4f lds_v4f(const lds_u8* p) { return *(const __attri
 
 // ---- the attention kernel ------------------------------------------------------
 //
-// A workgroup takes 16 NR rows (16, 32 or 64); its four waves split each tile:
-// for S^T every wave takes 16 of the 64 keys, for O^T a quarter of the latent
-// dimension, both for all rows. So K and V are read from LDS once a workgroup
-// however many rows there are (with waves split by rows they are read once a
-// wave, and LDS, not the matrix units, bounds 64 rows and more), and a
-// fragment feeds NR MFMAs. Q (R + P values of every row) and a quarter of O
-// stay in registers: 18 x 4 x NR + 8 x 4 x NR at 512 + 64, all of a SIMD's at
-// NR = 4. The row maxima and P go through LDS between the waves.
+// A workgroup takes MT row tiles of 16 rows (16, 32 or 64 rows); its four waves
+// split each key tile twice: for S^T a wave takes 16 of the 64 keys, for O^T a
+// quarter of the latent dimension, both for all rows. So K and V are read from
+// LDS once however many rows there are, and a fragment feeds MT MFMAs; S goes
+// through LDS as P between the two. Q (R + P values of every row) and a quarter
+// of O stay in registers: 72 MT and 32 MT of them at 512 + 64, so that 64 rows
+// take all of a SIMD's 512 for its one wave. Half of those are accumulation
+// registers, which MFMAs can read as operands; Q lies there, and its MFMAs are
+// written out, because the compiler would copy each fragment to an ordinary
+// register first (a tile of 64 rows 10000 clocks instead of 3500). With eight
+// waves instead, Q leaves no registers to read K fragments ahead with (9200).
 //
 // PAIR: the rows of a sequence fill two workgroups (65 rows and more); these
 // two take the same tiles at the same time on the same XCD, whose L2 then
 // brings a cached row from memory once for both.
-template <int R, int P, bool F8, int NR, int PAIR>
-__global__ __launch_bounds__(256, F8&& NR == 1 ? 2 : 1) void absorbed_kernel(const Absorbed p) {
+//
+// The reference point m of a row's exponentials only has to be near its maximum
+// (exp2 of up to 2^8 is far inside binary32 and bf16), so each wave compares its
+// own scores with it; only when one has grown past it by more than that do the
+// waves exchange maxima and rescale O, seldom after the first tile.
+
+// acc (+)= K fragment x Q fragment. The compiler does not know these for MFMAs,
+// so the waits it would put in stand here: two states between an ordinary
+// instruction that wrote the K fragment and the first product that reads it
+// (WAIT); a chain's next product comes MT - 1 others later; and qk_done waits
+// out the last ones before anything else touches the accumulators.
+template <bool ACC, bool FIRST, bool WAIT>
+__device__ __forceinline__ void mfma_qk(v4f& acc, const v8bf& k, const v8bf& q) {
+  if constexpr (WAIT && FIRST) {
+    if constexpr (ACC)
+      asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(acc) : "v"(k), "a"(q));
+    else
+      asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(acc) : "v"(k), "v"(q));
+  } else if constexpr (WAIT) {
+    if constexpr (ACC)
+      asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(acc) : "v"(k), "a"(q));
+    else
+      asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(acc) : "v"(k), "v"(q));
+  } else if constexpr (FIRST) {
+    if constexpr (ACC)
+      asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(acc) : "v"(k), "a"(q));
+    else
+      asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(acc) : "v"(k), "v"(q));
+  } else {
+    if constexpr (ACC)
+      asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(acc) : "v"(k), "a"(q));
+    else
+      asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(acc) : "v"(k), "v"(q));
+  }
+}
+template <int N>
+__device__ __forceinline__ void qk_done(v4f* s) {
+  if constexpr (N == 2)
+    asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1]));
+  else
+    asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3]));
+}
+
+// The kernel's arguments, read anew from the kernarg segment: what only the
+// ends of a segment need does not take scalar registers through its tiles.
+__device__ __forceinline__ Absorbed args_now() {
+#ifdef __HIP_DEVICE_COMPILE__
+  auto* k = (const __attribute__((address_space(4))) Absorbed*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(k));
+  return *k;
+#else
+  return Absorbed{};
+#endif
+}
+
+template <int R, int P, bool F8, int MT, int PAIR>
+__global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(const Absorbed p) {
   using T = Tile<R, P, F8>;
-  constexpr int ROWS = 16 * NR;       // of this workgroup
+  constexpr int ROWS = 16 * MT;       // of this workgroup
   constexpr int GROUP = ROWS * PAIR;  // of the row group that its pair shares
-  constexpr int KS = (R + P) / 32, RS = R / 32, DT = R / 64;  // 16x16x32 steps; d tiles of a wave
-  constexpr int PROW = 2 * kAbsKeys + 16;                      // bytes of a P row, padded off the banks' period
-  constexpr int SCL = 2 * T::BYTES, PBUF = SCL + (F8 ? 2 * 256 : 0), MAXB = PBUF + ROWS * PROW, FLAG = MAXB + 4 * ROWS * 4;
-  __shared__ __align__(1024) uint8_t smem[FLAG + 16];
+  constexpr int KS = (R + P) / 32, RS = R / 32, DT = R / 64;  // 16x16x32 steps; d tiles of a wave in O^T
+  constexpr int AKS = MT == 1 ? 0 : MT == 2 ? KS : KS < 16 ? KS : 16;  // steps whose Q lies in accumulation registers
+  constexpr int PROW = 2 * kAbsKeys + 16;  // bytes of a P row, padded off the banks' period
+  constexpr int SCL = 2 * T::BYTES, PBUF = SCL + (F8 ? 2 * 256 : 0), MAXB = PBUF + ROWS * PROW;
+  constexpr int FLAGS = MAXB + 4 * ROWS * 4;  // grown (even, odd tiles), bad page
+  constexpr bool QFITS = ROWS * 2 * (R + P) <= T::BYTES;  // Q on its way to registers: in the second buffer, or its own
+  constexpr int QOFF = QFITS ? T::BYTES : (FLAGS + 16 + 1023) / 1024 * 1024;
+  __shared__ __align__(1024) uint8_t smem[QFITS || MT == 1 ? FLAGS + 16 : QOFF + ROWS * 2 * (R + P)];
   lds_u8* lds = (lds_u8*)smem;
-  const int lane = (int)threadIdx.x % kWave, wave = (int)threadIdx.x / kWave;
-  const int q4 = lane / 16, c16 = lane % 16;
+  const int wave = wave_index();
   if (p.zero_tail)
     zero_uncovered(p.q_starts, p.batch, p.tokens, p.heads, R, p.out, p.ot, p.oh, p.lse, blockIdx.x, gridDim.x);
 
-  const int64_t units = total_units(p, GROUP);
-  const int64_t wgs = units < p.shares ? units : p.shares;
+  const int64_t units = count_items(
+      p.batch, [&](int b) { return absorbed_span(p, b); },
+      [&](const SeqSpan& q) { return (int64_t)row_groups(p, q, GROUP) * key_tiles(q); });
+  const int64_t shares = units < p.shares ? units : p.shares;
   // workgroups go to the 8 XCDs by blockIdx % 8: a pair's two are 8 apart
   const int member = PAIR == 2 ? (int)(blockIdx.x / 8 % 2) : 0;
   const int64_t g = PAIR == 2 ? blockIdx.x / 16 * 8 + blockIdx.x % 8 : blockIdx.x;
-  if (g >= wgs) return;
-  int64_t u = share_begin(units, g, wgs);
-  const int64_t u1 = share_begin(units, g + 1, wgs);
+  if (g >= shares) {
+    if (member == 0 && g < p.shares && threadIdx.x == 0) p.joints[g].valid = 0;
+    return;
+  }
+  int64_t u = share_begin(units, g, shares);
+  int left = share_size(units, g, shares);
+  bool joint = false;  // a joint of this share was written
+  const float c2 = uniform(p.scale * kLog2e);
 
-  // K reads: key krow, unit 4 j + q4 of a window of units that the swizzle
-  // stays in (16 units, 8 of an 8-bit row); the key part has one window.
-  const int krow = 16 * wave + c16;
-  int ka0 = krow * T::LROW + ((q4 ^ swz_key<F8>(krow)) * 16);
-  int kra0 = T::ROPE + krow * T::RROW + ((q4 ^ swz_rope<F8>(krow)) * 16);
-  // V^T reads: this lane's place in its group's block of keys 8 q4 .. 8 q4 + 7;
-  // unit u0 of the wave's quarter, whose other units differ from it in address
-  // bits that neither the key nor the lane touches
-  const int vkey = F8 ? 8 * q4 + c16 / 2 : 8 * q4 + c16 / 4;
-  const int u0 = F8 ? wave * DT : 2 * wave * DT + (c16 % 4) / 2;
-  int va0 = vkey * T::LROW + ((u0 ^ swz_key<F8>(vkey)) * 16) + (lane & 1) * 8;
-  const float c2 = p.scale * kLog2e;
-
-  while (u < u1) {
-    const Segment sg = next_segment(p, GROUP, u, u1, g);
-    u += sg.t_end - sg.t_begin;
+  while (left > 0) {
+    const Absorbed a = args_now();
+    const Segment sg = next_segment(a, GROUP, u, left);
     const SeqSpan& seq = sg.seq;
-    const int64_t rows = (int64_t)seq.n * p.heads;
-    const int64_t row0 = sg.row0 + member * ROWS;
+    const int rows = seq.n * a.heads;
+    const int row0 = sg.row0 + member * ROWS;
+    const bool whole = sg.t_begin == 0 && sg.t_end == sg.tiles;
+    // of a share's segments only the first can start inside a group's tiles and
+    // only the last can end inside them: two partial slots a share
+    const int64_t slot = 2 * g + (sg.t_begin == 0 ? 1 : 0);
+    if (!whole && sg.t_begin == 0) {
+      joint = true;
+      if (member == 0 && wave == 0 && lane_now() == 0) {
+        const int64_t last = share_of(opaque_uniform(units), u + sg.tiles - 1, shares);
+        a.joints[g] = Joint{seq.q0, rows, sg.row0, (int)last, 1};
+      }
+    }
+    u += sg.t_end - sg.t_begin;
+    left -= sg.t_end - sg.t_begin;
     if (PAIR == 2 && row0 >= rows) continue;  // the group's rows end with the other workgroup
-    // query token and head of this lane's row of row tile r (rows past the last repeat it and are not stored)
-    auto my_row = [&](int r, int& i, int& h) {
-      int row = (int)row0 + 16 * r + opaque(c16);
-      row = row < (int)rows ? row : (int)rows - 1;
-      i = row / p.heads;
-      h = row - i * p.heads;
+    // query token and head of row `at` of the workgroup (rows past the last repeat it and are not stored)
+    auto my_row = [&](int at, int& i, int& h) {
+      int row = row0 + at;
+      row = row < rows ? row : rows - 1;
+      const int heads = opaque_uniform(p.heads);
+      i = row / heads;
+      h = row - i * heads;
     };
-    const int lim_min = absorbed_limit(seq, (int)row0 / p.heads);
+    const int lim_min = absorbed_limit(seq, row0 / a.heads);
 
     Stager<R, P, F8> st;
-    st.begin(p, seq, sg.b);
-    __syncthreads();
-    if (threadIdx.x == 0) *(__attribute__((address_space(3))) int*)(lds + FLAG) = 0;
+    st.begin(p, seq, sg.b, wave);
     const bool any = seq.len > 0;
-    if (any) {
-      st.fetch(sg.t_begin);
-      st.issue(p, lds, lds + SCL);
-      if (sg.t_begin + 1 < sg.t_end) st.fetch(sg.t_begin + 1);
+    if (any) st.fetch(p, sg.t_begin);
+    lds_only_barrier();  // the last segment's accesses to LDS have ended
+    if (wave == 0) {
+      const int ln = lane_now();
+      if (ln < 3) *(lds_i32*)(lds + FLAGS + 4 * ln) = 0;
     }
-    // Q: B operand. bf16 rows: values 32 ks + 8 q4 ..; 8-bit rows: 64 (ks / 2) + 16 q4 + 8 (ks % 2) ..
-    v8bf qf[NR][KS];
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
+    // Q: B operand. bf16 rows: values 32 ks + 8 (lane / 16) ..; 8-bit rows are
+    // read 16 values a lane, two steps at once: 64 (ks / 2) + 16 (lane / 16) + 8 (ks % 2) ..
+    v8bf qf[MT][KS];
+    if constexpr (MT == 1) {
+      const int ql_ = lane_now(), qq = ql_ / 16;
       int i, h;
-      my_row(r, i, h);
-      const uint16_t* ql = p.ql + (seq.q0 + i) * p.qlt + h * p.qlh;
-      const uint16_t* qr = P ? p.qr + (seq.q0 + i) * p.qrt + h * p.qrh : nullptr;
+      my_row(ql_ % 16, i, h);
+      const uint16_t* ql = a.ql + (seq.q0 + i) * a.qlt + h * a.qlh;
+      const uint16_t* qr = P ? a.qr + (seq.q0 + i) * a.qrt + h * a.qrh : nullptr;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const int k = ks < RS ? ks : ks - RS;
-        const int d = F8 ? 64 * (k / 2) + 16 * q4 + 8 * (k % 2) : 32 * k + 8 * q4;
-        qf[r][ks] = *(const v8bf*)((ks < RS ? ql : qr) + d);
+        const int d = F8 ? 64 * (k / 2) + 16 * qq + 8 * (k % 2) : 32 * k + 8 * qq;
+        qf[0][ks] = *(const v8bf*)((ks < RS ? ql : qr) + d);
       }
-    }
-    float m[NR], l[NR];
-    v4f o[NR][DT];
+      lds_only_barrier();
+      if (any) {
+        st.start(p, lds + FLAGS + 8);
+        st.load_all(lds);
+        st.parts(p);
+        st.finish(lds, lds + SCL);
+        if (sg.t_begin + 1 < sg.t_end) st.fetch(p, sg.t_begin + 1);
+      }
+    } else {
+      // Through LDS, laid out as a bf16 tile: read straight into fragments, each
+      // wave would fetch every row in 64-byte pieces (15000 clocks for 64 rows).
+      // 16-bit tiles: in the second buffer, which the first iteration fills only
+      // once everyone has met at its barrier.
+      constexpr int QR = ROWS / 4;  // rows a wave brings
+      int i, h;
+      const uint32_t ln = (uint32_t)lane_now();
+      my_row(QR * wave + (int)(ln % QR), i, h);
+      const uint64_t ql = (uint64_t)(a.ql + (seq.q0 + i) * a.qlt + h * a.qlh);
+      const uint64_t qr = P ? (uint64_t)(a.qr + (seq.q0 + i) * a.qrt + h * a.qrh) : 0;
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
+      for (int k = 0; k < QR; ++k) {
+        const __amdgpu_buffer_rsrc_t row = __builtin_amdgcn_make_buffer_rsrc((void*)lane_value(ql, k), (short)0, 2 * R, kBufWord3);
+        const uint32_t x = (uint32_t)swz_key<false>(k) ^ (QR == 8 ? 8 * (wave & 1) : 0);
+        if (R == 512 || ln < R / 8)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(row, (__attribute__((address_space(3))) void*)(lds + QOFF + (QR * wave + k) * 2 * R),
+                                                   16, (ln ^ x) * 16, 0, 0, 0);
+      }
+      v4i qp[P > 0 ? QR / 8 : 1];
+      if constexpr (P > 0) {
+#pragma unroll
+        for (int k = 0; k < QR / 8; ++k)
+          qp[k] = *(const global_v4i*)(__shfl((unsigned long long)qr, 8 * k + (int)(ln / 8)) + (ln % 8) * 16);
+      }
+      lds_only_barrier();
+      if (any) {
+        st.start(p, lds + FLAGS + 8);
+        st.load_all(lds);
+        st.parts(p);
+      }
+      if constexpr (P > 0) {
+#pragma unroll
+        for (int k = 0; k < QR / 8; ++k) {
+          const uint32_t row = QR * wave + 8 * k + ln / 8;
+          *(__attribute__((address_space(3))) v4i*)(lds + QOFF + ROWS * 2 * R + row * 128 +
+                                                    ((ln % 8) ^ (uint32_t)swz_rope<false>(row)) * 16) = qp[k];
+        }
+      }
+      if (any) {
+        st.finish(lds, lds + SCL);
+        if (sg.t_begin + 1 < sg.t_end) st.fetch(p, sg.t_begin + 1);
+      }
+      loads_barrier();
+      const int ql_ = lane_now(), qq = ql_ / 16, qc = ql_ % 16;
+#pragma unroll
+      for (int r = 0; r < MT; ++r)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const int k = ks < RS ? ks : ks - RS;
+          const int unit = F8 ? 8 * (k / 2) + 2 * qq + k % 2 : 4 * k + qq;
+          qf[r][ks] = lds_v8bf(lds + QOFF + (ks < RS ? (16 * r + qc) * 2 * R + ((unit ^ swz_key<false>(qc)) * 16)
+                                                     : ROWS * 2 * R + (16 * r + qc) * 128 + ((unit ^ swz_rope<false>(qc)) * 16)));
+        }
+    }
+    float m[MT], l[MT];  // the rows' reference points, their sums over this lane's keys
+    v4f o[MT][DT];
+#pragma unroll
+    for (int r = 0; r < MT; ++r) {
       m[r] = -INFINITY;
       l[r] = 0.0f;
 #pragma unroll
@@ -349,92 +485,127 @@ __global__ __launch_bounds__(256, F8&& NR == 1 ? 2 : 1) void absorbed_kernel(con
 
     for (int tile = sg.t_begin; any && tile < sg.t_end; ++tile) {
       const int buf = (tile - sg.t_begin) & 1;
-      loads_barrier();
-      if (tile + 1 < sg.t_end) {
-        st.issue(p, lds + (buf ^ 1) * T::BYTES, lds + SCL + (buf ^ 1) * 256);
-        if (tile + 2 < sg.t_end) st.fetch(tile + 2);
-      }
+      const bool more = tile + 1 < sg.t_end;
+      loads_barrier();  // the tile has landed; everyone is done with the other buffer
+      if (more) st.start(p, lds + FLAGS + 8);
       const lds_u8* kb = lds + buf * T::BYTES;
-      // the addresses below are formed where they are used, an XOR each: hoisted out of the loop they would
-      // take the registers that Q and O need
-      const int ka = opaque(ka0), kra = opaque(kra0), va = opaque(va0);
-      v4f s[NR];
+      lds_u8* next = lds + (buf ^ 1) * T::BYTES;
+      // What depends on the lane is formed here, in each tile, and addresses
+      // where they are used, an XOR each: kept across the loop they would take
+      // the registers that Q and O need.
+      const int tl = lane_now(), tq = tl / 16, tc = tl % 16;
+      // K reads: key krow, unit 4 j + tq of a window of units that the swizzle
+      // stays in (16 units, 8 of an 8-bit row); the key part has one window
+      const int krow = 16 * wave + tc;
+      const int ka = krow * T::LROW + ((tq ^ swz_key<F8>(krow)) * 16);
+      const int kra = T::ROPE + krow * T::RROW + ((tq ^ swz_rope<F8>(krow)) * 16);
+      // One 16-byte read of K a step (an 8-bit row's serves two MFMAs), AHEAD
+      // steps before its MFMAs; the next tile's loads go between them.
+      constexpr int STEPS = F8 ? KS / 2 : KS, AHEAD = MT == 4 ? 3 : 4, RING = AHEAD + 1;
+      auto k_at = [&](int st_) {
+        if constexpr (F8) return st_ < RS / 2 ? (ka ^ ((st_ & 1) << 6)) + (st_ >> 1) * 128 : kra;
+        return st_ < RS ? (ka ^ ((st_ & 3) << 6)) + (st_ >> 2) * 256 : kra ^ ((st_ - RS) << 6);
+      };
+      v4f s[MT];
+      {
+        v4i kf[RING];
 #pragma unroll
-      for (int r = 0; r < NR; ++r) s[r] = v4f{0, 0, 0, 0};
-      if constexpr (F8) {
+        for (int i = 0; i < AHEAD && i < STEPS; ++i) kf[i] = lds_v4i(kb + k_at(i));
 #pragma unroll
-        for (int kk = 0; kk < KS / 2; ++kk) {
-          const int at = kk < RS / 2 ? (ka ^ ((kk & 1) << 6)) + (kk >> 1) * 128 : kra;
-          const v4i w = lds_v4i(kb + at);
-          const v8bf a0 = widen_e4m3(v2i{w[0], w[1]}), a1 = widen_e4m3(v2i{w[2], w[3]});
+        for (int i = 0; i < STEPS; ++i) {
+          if (i + AHEAD < STEPS) kf[(i + AHEAD) % RING] = lds_v4i(kb + k_at(i + AHEAD));
+          #pragma unroll
+          for (int k = i * 16 / STEPS; k < (i + 1) * 16 / STEPS; ++k)
+            if (more) st.load(next, k);
+
+          const v4i w = kf[i % RING];
+          auto products = [&](auto ks_, const v8bf& a) {
+            constexpr int ks = decltype(ks_)::value;
+            if constexpr (MT == 1) {
+              s[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[0][ks], ks == 0 ? v4f{0, 0, 0, 0} : s[0], 0, 0, 0);
+            } else {
 #pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            s[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, qf[r][2 * kk], s[r], 0, 0, 0);
-            s[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, qf[r][2 * kk + 1], s[r], 0, 0, 0);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const int at = ks < RS ? (ka ^ ((ks & 3) << 6)) + (ks >> 2) * 256 : kra ^ ((ks - RS) << 6);
-          const v8bf a = lds_v8bf(kb + at);
-#pragma unroll
-          for (int r = 0; r < NR; ++r) s[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[r][ks], s[r], 0, 0, 0);
-        }
-        if constexpr (NR == 4) {
-          __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            __builtin_amdgcn_sched_group_barrier(0x008, NR, 0);
-            if (ks + 4 < KS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-          }
+              for (int r = 0; r < MT; ++r) r == 0 ? mfma_qk<(ks < AKS), ks == 0, true>(s[r], a, qf[r][ks]) : mfma_qk<(ks < AKS), ks == 0, false>(s[r], a, qf[r][ks]);
+            }
+          };
+          unroll_at<STEPS>(i, [&](auto i_) {
+            constexpr int ii = decltype(i_)::value;
+            if constexpr (F8) {
+              products(std::integral_constant<int, 2 * ii>{}, widen_e4m3(v2i{w[0], w[1]}));
+              products(std::integral_constant<int, 2 * ii + 1>{}, widen_e4m3(v2i{w[2], w[3]}));
+            } else {
+              products(std::integral_constant<int, ii>{}, __builtin_bit_cast(v8bf, w));
+            }
+          });
         }
       }
-      // lane: row c16 of each row tile, keys 16 wave + 4 q4 + i
+      if constexpr (MT > 1) qk_done<MT>(s);
+      if (more) st.parts(p);  // not before: their registers are K's until here
+      __builtin_amdgcn_sched_barrier(0);
+      // lane: row tc of each row tile, keys 16 wave + 4 tq + i
       if constexpr (F8) {
-        const v4f sc = lds_v4f(lds + SCL + buf * 256 + (16 * wave + 4 * q4) * 4);
+        const v4f sc = lds_v4f(lds + SCL + buf * 256 + (16 * wave + 4 * tq) * 4);
 #pragma unroll
-        for (int r = 0; r < NR; ++r)
+        for (int r = 0; r < MT; ++r)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[r][i] *= sc[i];
       }
       if ((tile + 1) * kAbsKeys > lim_min) {
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
+        for (int r = 0; r < MT; ++r) {
           int qi, h;
-          my_row(r, qi, h);
-          const int lim = absorbed_limit(seq, qi) - (tile * kAbsKeys + 16 * wave + 4 * q4);
+          my_row(16 * r + lane_now() % 16, qi, h);
+          const int lim = absorbed_limit(seq, qi) - (tile * kAbsKeys + 16 * wave + 4 * tq);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (i >= lim) s[r][i] = -INFINITY;
         }
       }
-#pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        float top = fmaxf(fmaxf(s[r][0], s[r][1]), fmaxf(s[r][2], s[r][3]));
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        if (lane < 16) *(__attribute__((address_space(3))) float*)(lds + MAXB + (wave * ROWS + 16 * r + lane) * 4) = top;
-      }
-      lds_only_barrier();
-      // The reference point m only has to be near the row's maximum (exp2 of up
-      // to 2^8 is far inside binary32 and bf16): O is rescaled when some row's
-      // maximum has grown past it by more than that, seldom after the first
-      // tile. All waves see the same maxima and decide alike.
-      float top[NR];
+      float top[MT];
       bool grown = false;
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        top[r] = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          top[r] = fmaxf(top[r], *(__attribute__((address_space(3))) float*)(lds + MAXB + (w * ROWS + 16 * r + c16) * 4));
+      for (int r = 0; r < MT; ++r) {
+        top[r] = fmaxf(fmaxf(s[r][0], s[r][1]), fmaxf(s[r][2], s[r][3]));
         grown = grown || (top[r] - m[r]) * c2 > 8.0f;
       }
-      if (__any(grown)) {
+      if (__any(grown)) *(lds_i32*)(lds + FLAGS + 4 * buf) = 1;  // every lane writes the same
+      float sum[MT];
+      auto weights = [&]() {
+        const int wl = lane_now(), wq = wl / 16, wc = wl % 16;
+        v4f sc = v4f{1, 1, 1, 1};
+        if constexpr (F8) sc = lds_v4f(lds + SCL + buf * 256 + (16 * wave + 4 * wq) * 4);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          const float mn = fmaxf(m[r], top[r]);
+        for (int r = 0; r < MT; ++r) {
+          const float mc = m[r] == -INFINITY ? 0.0f : m[r] * c2;
+          float e[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i], c2, -mc));
+          sum[r] = (e[0] + e[1]) + (e[2] + e[3]);
+          if constexpr (F8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] *= sc[i];
+          }
+          *(__attribute__((address_space(3))) v2i*)(lds + PBUF + (16 * r + wc) * PROW + (16 * wave + 4 * wq) * 2) =
+              v2i{(int)pack_bf16(e[0], e[1]), (int)pack_bf16(e[2], e[3])};
+        }
+      };
+      weights();
+      lds_only_barrier();
+      if (__builtin_amdgcn_readfirstlane(*(lds_i32*)(lds + FLAGS + 4 * buf))) {
+        // some row's maximum has grown: exchange maxima, rescale, form P again
+        const int rl = lane_now();
+#pragma unroll
+        for (int r = 0; r < MT; ++r) {
+          top[r] = fmaxf(top[r], __shfl_xor(top[r], 16));
+          top[r] = fmaxf(top[r], __shfl_xor(top[r], 32));
+          if (rl < 16) *(lds_f32*)(lds + MAXB + (wave * ROWS + 16 * r + rl) * 4) = top[r];
+        }
+        lds_only_barrier();
+#pragma unroll
+        for (int r = 0; r < MT; ++r) {
+          float mn = m[r];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) mn = fmaxf(mn, *(lds_f32*)(lds + MAXB + (w * ROWS + 16 * r + rl % 16) * 4));
           const float a = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[r] - mn) * c2);
           m[r] = mn;
           l[r] *= a;
@@ -443,84 +614,99 @@ __global__ __launch_bounds__(256, F8&& NR == 1 ? 2 : 1) void absorbed_kernel(con
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[r][t][i] *= a;
         }
+        weights();
+        lds_only_barrier();
       }
-      v4f sc = v4f{1, 1, 1, 1};
-      if constexpr (F8) sc = lds_v4f(lds + SCL + buf * 256 + opaque((16 * wave + 4 * q4) * 4));
+      // V^T reads: this lane's place in its group's block of keys 8 vq .. 8 vq + 7;
+      // unit u0 of the wave's quarter, whose other units differ from it in address
+      // bits that neither the key nor the lane touches
+      const int vl = lane_now(), vq = vl / 16, vc = vl % 16;
+      const int vkey = F8 ? 8 * vq + vc / 2 : 8 * vq + vc / 4;
+      const int u0 = F8 ? wave * DT : 2 * wave * DT + (vc % 4) / 2;
+      const int va = vkey * T::LROW + ((u0 ^ swz_key<F8>(vkey)) * 16) + (vl & 1) * 8;
+      if (wave == 0) *(lds_i32*)(lds + FLAGS + 4 * (buf ^ 1)) = 0;  // all have read it before this tile's barriers
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        const float mc = m[r] == -INFINITY ? 0.0f : m[r] * c2;
-        float e[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i], c2, -mc));
-          l[r] += e[i];
-          if constexpr (F8) e[i] *= sc[i];
-        }
-        *(__attribute__((address_space(3))) v2i*)(lds + PBUF + (16 * r + c16) * PROW + (16 * wave + 4 * q4) * 2) =
-            v2i{(int)pack_bf16(e[0], e[1]), (int)pack_bf16(e[2], e[3])};
-      }
-      lds_only_barrier();
-#pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) {
-        v8bf pf[NR];
-#pragma unroll
-        for (int r = 0; r < NR; ++r) pf[r] = lds_v8bf(lds + PBUF + (16 * r + c16) * PROW + (32 * s2 + 8 * q4) * 2);
-#pragma unroll
-        for (int t = 0; t < DT; ++t) {
-          v8bf vf;
+      for (int r = 0; r < MT; ++r) l[r] += sum[r];
+      // V fragments are read ahead of their MFMAs (the schedule is pinned: left to
+      // itself the compiler reads each where it is used, and every d tile waits out
+      // the LDS latency); the other half of the next tile's loads goes between.
+      {
+        constexpr int VN = 2 * DT, VAHEAD = 2, VRING = VAHEAD + 1;
+        v4s vlo[VRING], vhi[VRING];
+        v2i v8[VRING];
+        auto v_read = [&](int n) {
+          const int s2 = n / DT, t = n % DT;
           if constexpr (F8) {
-            vf = widen_e4m3(read_tr8(kb + (va ^ (t << 4)) + 32 * s2 * T::LROW));
+            v8[n % VRING] = read_tr8(kb + (va ^ (t << 4)) + 32 * s2 * T::LROW);
           } else {
-            const v4s lo = read_tr16(kb + (va ^ (t << 5)) + 32 * s2 * T::LROW);
-            const v4s hi = read_tr16(kb + (va ^ ((t << 5) | 16)) + (32 * s2 + 4) * T::LROW);  // keys + 4: swizzle bit 0
-            vf = join_tr16(lo, hi);
+            vlo[n % VRING] = read_tr16(kb + (va ^ (t << 5)) + 32 * s2 * T::LROW);
+            vhi[n % VRING] = read_tr16(kb + (va ^ ((t << 5) | 16)) + (32 * s2 + 4) * T::LROW);  // keys + 4: swizzle bit 0
           }
+        };
+        v8bf pf[MT];
 #pragma unroll
-          for (int r = 0; r < NR; ++r) o[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[r], o[r][t], 0, 0, 0);
+        for (int r = 0; r < MT; ++r) pf[r] = lds_v8bf(lds + PBUF + (16 * r + vc) * PROW + (8 * vq) * 2);
+#pragma unroll
+        for (int n = 0; n < VAHEAD; ++n) v_read(n);
+#pragma unroll
+        for (int n = 0; n < VN; ++n) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (n + VAHEAD < VN) v_read(n + VAHEAD);
+          __builtin_amdgcn_sched_barrier(0);
+          const v8bf vf = F8 ? widen_e4m3(v8[n % VRING]) : join_tr16(vlo[n % VRING], vhi[n % VRING]);
+#pragma unroll
+          for (int r = 0; r < MT; ++r) {
+            o[r][n % DT] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[r], o[r][n % DT], 0, 0, 0);
+            if (n == DT - 1) pf[r] = lds_v8bf(lds + PBUF + (16 * r + vc) * PROW + (32 + 8 * vq) * 2);
+          }
         }
+      }
+      if (more) {
+        st.finish(next, lds + SCL + (buf ^ 1) * 256);
+        if (tile + 2 < sg.t_end) st.fetch(p, tile + 2);
       }
     }
 
-    if (__any(st.bad) && lane == 0) *(__attribute__((address_space(3))) int*)(lds + FLAG) = 1;
-    // the row sums: lanes of a row hold its keys 4 q4 .. of each wave's 16
+    // the row sums: lanes of a row hold its keys 4 (lane / 16) .. of each wave's 16
+    const Absorbed e = args_now();
+    const int el = lane_now(), eq = el / 16, ec = el % 16;
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
+    for (int r = 0; r < MT; ++r) {
       l[r] += __shfl_xor(l[r], 16);
       l[r] += __shfl_xor(l[r], 32);
+      if (el < 16) *(lds_f32*)(lds + MAXB + (wave * ROWS + 16 * r + el) * 4) = l[r];
     }
-    __syncthreads();
+    lds_only_barrier();
+    const bool poisoned = *(lds_i32*)(lds + FLAGS + 8) != 0;
 #pragma unroll
-    for (int r = 0; r < NR; ++r)
-      if (lane < 16) *(__attribute__((address_space(3))) float*)(lds + MAXB + (wave * ROWS + 16 * r + lane) * 4) = l[r];
-    __syncthreads();
-    const bool poisoned = *(__attribute__((address_space(3))) int*)(lds + FLAG) != 0;
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
+    for (int r = 0; r < MT; ++r) {
       float sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) sum += *(__attribute__((address_space(3))) float*)(lds + MAXB + (w * ROWS + 16 * r + c16) * 4);
+      for (int w = 0; w < 4; ++w) sum += *(lds_f32*)(lds + MAXB + (w * ROWS + 16 * r + ec) * 4);
       if (poisoned) sum = __uint_as_float(0x7fc00000u);
+      // a row that sees no key has a sum of 0: its output is 0 and its lse -inf
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      if (!sg.whole) {
-        if (wave == 0 && lane < 16)
-          p.part_lse[sg.slot * GROUP + member * ROWS + 16 * r + lane] = sum == 0.0f ? -INFINITY : __builtin_fmaf(m[r], c2, log2f(sum));
-        float4* po = (float4*)p.part_o + ((sg.slot * (NR * PAIR) + member * NR + r) * (R / 16) + wave * DT) * 64 + lane;
+      if (!whole) {
+        if (wave == 0 && el < 16)
+          e.part_lse[slot * GROUP + member * ROWS + 16 * r + el] = sum == 0.0f ? -INFINITY : __builtin_fmaf(m[r], c2, log2f(sum));
+        float4* po = (float4*)e.part_o + ((slot * (MT * PAIR) + member * MT + r) * (R / 16) + wave * DT) * 64 + el;
 #pragma unroll
         for (int t = 0; t < DT; ++t) po[t * 64] = make_float4(o[r][t][0] * inv, o[r][t][1] * inv, o[r][t][2] * inv, o[r][t][3] * inv);
         continue;
       }
-      if (row0 + 16 * r + c16 >= rows) continue;
+      if (row0 + 16 * r + ec >= rows) continue;
       int qi, h;
-      my_row(r, qi, h);
+      my_row(16 * r + ec, qi, h);
       const int64_t token = seq.q0 + qi;
-      if (p.lse && wave == 0 && lane < 16)
-        p.lse[token * p.heads + h] = sum == 0.0f ? -INFINITY : __builtin_fmaf(m[r], p.scale, logf(sum));
-      uint16_t* orow = p.out + token * p.ot + h * p.oh + wave * (R / 4) + 4 * q4;
+      if (e.lse && wave == 0 && el < 16)
+        e.lse[token * e.heads + h] = sum == 0.0f ? -INFINITY : __builtin_fmaf(m[r], e.scale, logf(sum));
+      uint16_t* orow = e.out + token * e.ot + h * e.oh + wave * (16 * DT) + 4 * eq;
 #pragma unroll
       for (int t = 0; t < DT; ++t)
         *(uint2*)(orow + 16 * t) = make_uint2(pack_bf16(o[r][t][0] * inv, o[r][t][1] * inv), pack_bf16(o[r][t][2] * inv, o[r][t][3] * inv));
     }
   }
+  if (!joint && member == 0 && wave == 0 && lane_now() == 0) p.joints[g].valid = 0;
 }
 
 // ---- joining the partial results ------------------------------------------------
@@ -534,28 +720,12 @@ __global__ __launch_bounds__(256) void absorbed_combine_kernel(const Absorbed p)
   __shared__ float sm[4][64], sl[4][64];
   __shared__ float4 so[4][PIECES][64];
   const int lane = (int)threadIdx.x % kWave, wave = (int)threadIdx.x / kWave;
-  const int64_t units = total_units(p, ROWS);
-  const int64_t wgs = units < p.shares ? units : p.shares;
   const int strip = (int)(blockIdx.x % STRIPS);
-  int64_t group0;
-  // sequence of this row group, and its first unit
-  const int64_t item = blockIdx.x / STRIPS;
-  const int b = find_sequence(
-      p.batch, item, [&](int s) { return (int64_t)row_groups(p, absorbed_span(p, s), ROWS); }, &group0);
-  if (b < 0) return;
-  const SeqSpan seq = absorbed_span(p, b);
-  const int tiles = key_tiles(seq);
-  int64_t before = 0;
-  for (int s = lane; s < b; s += kWave) {
-    const SeqSpan q = absorbed_span(p, s);
-    before += (int64_t)row_groups(p, q, ROWS) * key_tiles(q);
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o);
-  const int64_t first = before + (item - group0) * tiles;
-  const int64_t g0 = share_of(units, first, wgs), g1 = share_of(units, first + tiles - 1, wgs);
-  if (g0 == g1) return;  // one workgroup had all tiles and wrote the rows itself
-  const int64_t row = (item - group0) * ROWS + strip * 16 + lane % 16;
+  const int64_t g0 = blockIdx.x / STRIPS;
+  const Joint j = p.joints[g0];
+  const int row = j.row0 + strip * 16 + lane % 16;
+  if (!j.valid || j.row0 + strip * 16 >= j.rows) return;
+  const int64_t g1 = j.last;
   const int piece0 = (int)blockIdx.y * PIECES;
 
   float m = -INFINITY, l = 0.0f;
@@ -597,10 +767,10 @@ __global__ __launch_bounds__(256) void absorbed_combine_kernel(const Absorbed p)
     w[v] = sl[v][lane] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(sm[v][lane] - top);
     total += w[v] * sl[v][lane];
   }
-  if (row >= (int64_t)seq.n * p.heads) return;
+  if (row >= j.rows) return;
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  const int64_t token = seq.q0 + row / p.heads;
-  const int h = (int)(row % p.heads);
+  const int64_t token = j.q0 + row / p.heads;
+  const int h = row % p.heads;
   if (p.lse && piece0 == 0 && wave == 0 && lane < 16)
     p.lse[token * p.heads + h] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
   uint16_t* orow = p.out + token * p.ot + h * p.oh + 4 * (lane / 16);
@@ -624,7 +794,7 @@ struct AbsPlan {
   int rows;        // of a row group: 16, 32, 64, or 128 in two workgroups
   int64_t groups;  // upper bound of the batch's row groups
   int64_t shares;  // the units are divided into
-  size_t lse_bytes, bytes;
+  size_t joint_bytes, lse_bytes, bytes;
 };
 
 AbsPlan absorbed_plan(const fcmoe_absorbed_args* a) {
@@ -640,8 +810,9 @@ AbsPlan absorbed_plan(const fcmoe_absorbed_args* a) {
   const int64_t slots = pl.rows == 128 ? cus / 2 : (int64_t)cus * (a->cache.e4m3 && pl.rows == 16 ? 2 : 1);
   const int64_t most = pl.groups * (a->table_width > 0 ? ceil_div(a->table_width * a->cache.page_size, kAbsKeys) : 1);
   pl.shares = most < slots ? (most > 0 ? most : 1) : slots;
+  pl.joint_bytes = (size_t)round_up(pl.shares * (int64_t)sizeof(Joint), 256);
   pl.lse_bytes = (size_t)round_up(2 * pl.shares * pl.rows * 4, 256);
-  pl.bytes = pl.lse_bytes + (size_t)(2 * pl.shares) * (size_t)pl.rows * (size_t)a->cache.latent_dim * 4;
+  pl.bytes = pl.joint_bytes + pl.lse_bytes + (size_t)(2 * pl.shares) * (size_t)pl.rows * (size_t)a->cache.latent_dim * 4;
   return pl;
 }
 
@@ -661,7 +832,7 @@ void absorbed_launch(const Absorbed& p, const AbsPlan& pl, hipStream_t stream) {
 template <int R>
 void combine_launch(const Absorbed& p, const AbsPlan& pl, hipStream_t stream) {
   const dim3 b(256);
-  const unsigned g = (unsigned)pl.groups;
+  const unsigned g = (unsigned)pl.shares;
   if (pl.rows == 128)
     hipLaunchKernelGGL((absorbed_combine_kernel<R, 128, 4>), dim3(g * 8, R / 64), b, 0, stream, p);
   else if (pl.rows == 64)
@@ -681,6 +852,9 @@ int check_absorbed(const fcmoe_absorbed_args* a) {
       a->tokens * a->heads > INT32_MAX / 2 || a->table_width < 0 || a->table_width > INT32_MAX ||
       a->page_table_stride < 0)
     return fail(FCMOE_EINVAL, "absorbed_attention: bad shape");
+  // units are counted in 32 bits a sequence
+  if (ceil_div(a->tokens * a->heads, 16) + a->batch > INT32_MAX / (ceil_div(a->table_width * a->cache.page_size, kAbsKeys) + 1))
+    return fail(FCMOE_EINVAL, "absorbed_attention: too many rows for a page table of this reach");
   if (!a->query_starts && a->tokens != a->batch)
     return fail(FCMOE_EINVAL, "absorbed_attention: without query_starts there is one token a sequence");
   return FCMOE_OK;
@@ -721,9 +895,13 @@ extern "C" int fcmoe_absorbed_attention(const fcmoe_absorbed_args* a, hipStream_
   p.tokens = a->tokens, p.batch = (int)a->batch, p.heads = (int)a->heads;
   p.scale = a->scale;
   p.out = a->out, p.ot = a->out_token_stride, p.oh = a->out_head_stride, p.lse = a->lse;
-  p.part_lse = (float*)a->workspace;
-  p.part_o = (float*)((char*)a->workspace + pl.lse_bytes);
+  p.joints = (Joint*)a->workspace;
+  p.part_lse = (float*)((char*)a->workspace + pl.joint_bytes);
+  p.part_o = (float*)((char*)a->workspace + pl.joint_bytes + pl.lse_bytes);
   p.shares = (int)pl.shares;
+  p.page_shift = -1;
+  for (int i = 0; i <= 20; ++i)
+    if (p.c.page_size == (int64_t)1 << i) p.page_shift = i;
   p.zero_tail = a->zero_uncovered && a->query_starts;
   const bool f8 = a->cache.e4m3 != 0;
   if (a->cache.latent_dim == 512) {

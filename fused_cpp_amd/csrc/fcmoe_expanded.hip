@@ -94,10 +94,11 @@ __global__ __launch_bounds__(kExpWaves * kWave, 2) void expanded_kernel(const Ex
   const int head = (int)(item % p.heads);
   const int64_t block = p.blocks - 1 - item / p.heads;
   int64_t before;
+  SeqSpan seq;
   const int b = find_sequence(
-      p.batch, block, [&](int s) { return (int64_t)(expanded_span(p, s).n + kExpRows - 1) / kExpRows; }, &before);
+      p.batch, block, [&](int s) { return expanded_span(p, s); },
+      [](const SeqSpan& s) { return ((int64_t)s.n + kExpRows - 1) / kExpRows; }, &seq, &before);
   if (b < 0) return;
-  const SeqSpan seq = expanded_span(p, b);
   const int i0 = (int)(block - before) * kExpRows;
   const int wave_i0 = i0 + 32 * wave;
   const bool live = wave_i0 < seq.n;
@@ -281,10 +282,11 @@ __global__ __launch_bounds__(kExpWaves * kWave) void expanded_combine_kernel(con
   const int head = (int)(item % p.heads);
   const int64_t block = p.blocks - 1 - item / p.heads;
   int64_t before;
+  SeqSpan seq;
   const int b = find_sequence(
-      p.batch, block, [&](int s) { return (int64_t)(expanded_span(p, s).n + kExpRows - 1) / kExpRows; }, &before);
+      p.batch, block, [&](int s) { return expanded_span(p, s); },
+      [](const SeqSpan& s) { return ((int64_t)s.n + kExpRows - 1) / kExpRows; }, &seq, &before);
   if (b < 0) return;
-  const SeqSpan seq = expanded_span(p, b);
   const int i = (int)(block - before) * kExpRows + 32 * wave + lane % 32;
   if (i >= seq.n) return;
   const int64_t step = p.blocks * p.heads * kExpWaves;

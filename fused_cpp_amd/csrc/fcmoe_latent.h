@@ -104,6 +104,46 @@ __device__ __forceinline__ float other_half(float v) {
   return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
+// A value the compiler cannot see through: what depends on it is formed after this point.
+__device__ __forceinline__ int opaque(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+__device__ __forceinline__ int64_t opaque_uniform(int64_t v) {
+  asm volatile("" : "+s"(v));
+  return v;
+}
+__device__ __forceinline__ int opaque_uniform(int v) {
+  asm volatile("" : "+s"(v));
+  return v;
+}
+// The lane's number, formed anew: what depends on it is neither kept in a register nor hoisted past this point.
+__device__ __forceinline__ int lane_now() {
+  int l;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+  return l;
+}
+// A value that is the same in all lanes, in scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint64_t)v >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ float uniform(float v) {
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
+}
+
+// The wave's number in its workgroup, known to be the same in all its lanes.
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave); }
+// Lane l's value, in scalar registers (l the same for the whole wave).
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, int l) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l);
+  return ((uint64_t)hi << 32) | lo;
+}
+
 // Lengths that the device reads are bounded here, so that no value of them
 // leads a kernel outside the tensors the host has checked.
 struct SeqSpan {
@@ -117,38 +157,61 @@ __device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) {
   return v < lo ? lo : v > hi ? hi : v;
 }
 
-// Inclusive sum over the wave's lanes.
+// Inclusive sum over the wave's lanes: DPP moves within rows of 16, then the
+// rows' ends to the rows behind them (an LDS-crossbar scan costs six dependent
+// round trips).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t add_dpp(int64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)((uint64_t)v >> 32), CTRL, ROWS, 0xf, true);
+  return v + (int64_t)(((uint64_t)hi << 32) | lo);
+}
 __device__ __forceinline__ int64_t wave_scan(int64_t v) {
-  const int lane = (int)threadIdx.x % kWave;
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int64_t u = __shfl_up(v, o);
-    if (lane >= o) v += u;
-  }
+  v = add_dpp<0x111, 0xf>(v);  // row_shr:1
+  v = add_dpp<0x112, 0xf>(v);  // row_shr:2
+  v = add_dpp<0x114, 0xf>(v);  // row_shr:4
+  v = add_dpp<0x118, 0xf>(v);  // row_shr:8
+  v = add_dpp<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+  v = add_dpp<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
   return v;
 }
 
-// Finds the sequence that item `item` (0 <= item) falls into, where sequence b
-// holds count(b) items: its index, the items before it, and -1 past the last.
-// Every lane of the wave takes part and gets the same answer.
-template <typename F>
-__device__ __forceinline__ int find_sequence(int batch, int64_t item, F count, int64_t* before) {
-  const int lane = (int)threadIdx.x % kWave;
+// Finds the sequence that item `item` (0 <= item) falls into, where a sequence
+// with span s holds count(s) items: its index and span and the items before it;
+// -1 past the last. The whole wave takes part and gets the same answer.
+template <typename S, typename F>
+__device__ __forceinline__ int find_sequence(int batch, int64_t item, S span, F count, SeqSpan* found, int64_t* before) {
   int64_t base = 0;
   for (int b0 = 0; b0 < batch; b0 += kWave) {
-    const int b = b0 + lane;
-    const int64_t mine = b < batch ? count(b) : 0;
+    const int b = b0 + lane_now();
+    SeqSpan s{};
+    int64_t mine = 0;
+    if (b < batch) {
+      s = span(b);
+      mine = count(s);
+    }
     const int64_t upto = base + wave_scan(mine);
     const uint64_t hit = __ballot(upto > item);
     if (hit) {
       const int first = __ffsll((unsigned long long)hit) - 1;
-      *before = __shfl(upto - mine, first);
+      found->q0 = (int64_t)lane_value((uint64_t)s.q0, first);
+      found->k0 = (int64_t)lane_value((uint64_t)s.k0, first);
+      found->n = __builtin_amdgcn_readlane(s.n, first);
+      found->len = __builtin_amdgcn_readlane(s.len, first);
+      *before = (int64_t)lane_value((uint64_t)(upto - mine), first);
       return b0 + first;
     }
-    base = __shfl(upto, kWave - 1);
+    base = (int64_t)lane_value((uint64_t)upto, kWave - 1);
   }
   *before = base;
   return -1;
+}
+// Items of the whole batch.
+template <typename S, typename F>
+__device__ __forceinline__ int64_t count_items(int batch, S span, F count) {
+  int64_t sum = 0;
+  for (int b = lane_now(); b < batch; b += kWave) sum += count(span(b));
+  return (int64_t)lane_value((uint64_t)wave_scan(sum), kWave - 1);
 }
 
 // Tokens that no sequence holds (before the first start, behind the last)
