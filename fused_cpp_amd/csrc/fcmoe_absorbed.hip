@@ -33,11 +33,14 @@ constexpr int kAbsKeys = 64;  // keys of a tile
 constexpr int kBufWord3 = 0x00020000;  // raw buffer resource word 3 for gfx9: 32-bit data format, no swizzle
 
 // A row group whose tiles end up with several shares: left by the share that
-// has its first tile for the launch that joins the partial results.
+// has its first tile for the launch that joins the partial results. Kept by
+// group where there are no more groups than shares (every group's is written,
+// most not valid), else by share (of which at most one group's last tile lies
+// beyond it).
 struct Joint {
   int64_t q0;
-  int rows, row0;  // of the sequence; first of the group
-  int last;        // share with the group's last tile
+  int rows, row0;   // of the sequence; first of the group
+  int first, last;  // shares with the group's first and last tile
   int valid;
 };
 
@@ -59,7 +62,9 @@ struct Absorbed {
   float* lse;
   float* part_o;    // [2 * shares slots][rows * R]
   float* part_lse;  // [2 * shares slots][rows], base 2
-  Joint* joints;    // [shares]
+  Joint* joints;    // [groups] or [shares]
+  int* groups;      // [1] groups of the batch
+  int by_group;
   int shares;
   int page_shift;  // log2 of a page size that is a power of two, else -1
   int zero_tail;
@@ -85,6 +90,11 @@ __device__ __forceinline__ int row_groups(const Absorbed& p, const SeqSpan& s, i
 }
 // Tiles of a row group; at least one, so that a sequence without keys still gets its rows written.
 __device__ __forceinline__ int key_tiles(const SeqSpan& s) { return s.len > 0 ? (s.len + kAbsKeys - 1) / kAbsKeys : 1; }
+// Units of a row group: its tiles, and ahead of them what bringing its queries
+// in costs in tiles' time (96 sequences of up to 6000 8-bit keys, 32 rows each:
+// 82 us without it, 70 with).
+constexpr int kGroupCost = 2;
+__device__ __forceinline__ int group_units(const SeqSpan& s) { return key_tiles(s) + kGroupCost; }
 
 __device__ __forceinline__ int absorbed_limit(const SeqSpan& s, int i) {
   const int v = s.len - s.n + i + 1;
@@ -108,6 +118,7 @@ struct Segment {
   int row0;            // first row of the group
   int t_begin, t_end;  // tiles
   int tiles;           // of the group
+  int units, ahead;
 };
 
 // The segment that starts at unit u, `left` units before the end of its share.
@@ -116,13 +127,16 @@ __device__ __forceinline__ Segment next_segment(const Absorbed& p, int rows, int
   int64_t before;
   s.b = find_sequence(
       p.batch, u, [&](int b) { return absorbed_span(p, b); },
-      [&](const SeqSpan& q) { return (int64_t)row_groups(p, q, rows) * key_tiles(q); }, &s.seq, &before);
+      [&](const SeqSpan& q) { return (int64_t)row_groups(p, q, rows) * group_units(q); }, &s.seq, &before);
   s.tiles = key_tiles(s.seq);
-  const uint32_t rel = (uint32_t)(u - before);  // a sequence's units: its row groups times its tiles
-  const uint32_t group = rel / (uint32_t)s.tiles;
-  s.t_begin = uniform((int)(rel - group * (uint32_t)s.tiles));
-  s.t_end = uniform(s.t_begin + min(s.tiles - s.t_begin, left));
+  const uint32_t rel = (uint32_t)(u - before);  // among the sequence's units
+  const uint32_t per = (uint32_t)group_units(s.seq), group = rel / per;
+  const int first = (int)(rel - group * per);  // among the group's
+  s.units = uniform(min((int)per - first, left));
+  s.t_begin = uniform(max(first - kGroupCost, 0));
+  s.t_end = uniform(max(first + s.units - kGroupCost, 0));
   s.row0 = uniform((int)group * rows);
+  s.ahead = uniform(kGroupCost + s.tiles - 1 - first);  // units from u to the group's last
   return s;
 }
 
@@ -167,15 +181,16 @@ template <int R, int P, bool F8>
 struct Stager {
   using T = Tile<R, P, F8>;
   const int32_t* table;
-  int wave, last_key;  // last_key: of the sequence
+  int wave, turn, last_key;  // last_key: of the sequence
   int32_t id;
   int in;
   uint64_t lat;  // the tile being brought in
   v4i part[P > 0 ? T::RLOADS : 1];
   float scale;
 
-  __device__ __forceinline__ void begin(const Absorbed& p, const SeqSpan& s, int b, int w) {
+  __device__ __forceinline__ void begin(const Absorbed& p, const SeqSpan& s, int b, int w, int member) {
     wave = w;
+    turn = 8 * member;
     table = p.table + (int64_t)b * p.table_stride;
     last_key = s.len - 1;
   }
@@ -206,13 +221,18 @@ struct Stager {
     }
     if constexpr (F8) scale = p.c.scale[id * p.c.scale_page_stride + in];
   }
-  // The latent row of key u (0 .. 15) to its place in buffer `dst`.
+  // The latent row of key u ^ turn (u 0 .. 15, turn 0 or 8) to its place in
+  // buffer `dst`. A CU takes what its L2 lacks at some 10 bytes a clock, what
+  // it has at 60: the two workgroups that share keys bring the halves of their
+  // 16 in opposite orders, so that each finds one half fetched by the other.
   __device__ __forceinline__ void load(lds_u8* dst, int u) const {
     const uint32_t ln = (uint32_t)lane_now();
-    const __amdgpu_buffer_rsrc_t row = __builtin_amdgcn_make_buffer_rsrc((void*)lane_value(lat, u), (short)0, T::LROW, kBufWord3);
+    const int k = u ^ turn;
+    const __amdgpu_buffer_rsrc_t row = __builtin_amdgcn_make_buffer_rsrc((void*)lane_value(lat, k), (short)0, T::LROW, kBufWord3);
+    const uint32_t x = (uint32_t)swz_key<F8>(u) ^ (uint32_t)(F8 ? turn / 2 : turn);
     if (T::UNITS == 64 || ln < T::UNITS)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(row, (__attribute__((address_space(3))) void*)(dst + (16 * wave + u) * T::LROW), 16,
-                                               (ln ^ (uint32_t)swz_key<F8>(u)) * 16, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(row, (__attribute__((address_space(3))) void*)(dst + (16 * wave + k) * T::LROW), 16,
+                                               (ln ^ x) * 16, 0, 0, 0);
   }
   __device__ __forceinline__ void load_all(lds_u8* dst) const {
 #pragma unroll
@@ -261,7 +281,7 @@ __device__ __forceinline__ v4f lds_v4f(const lds_u8* p) { return *(const __attri
 // take all of a SIMD's 512 for its one wave. Half of those are accumulation
 // registers, which MFMAs can read as operands; Q lies there, and its MFMAs are
 // written out, because the compiler would copy each fragment to an ordinary
-// register first (a tile of 64 rows 10000 clocks instead of 3500). With eight
+// register first (a tile of 64 rows took 10000 clocks, now 6900). With eight
 // waves instead, Q leaves no registers to read K fragments ahead with (9200).
 //
 // PAIR: the rows of a sequence fill two workgroups (65 rows and more); these
@@ -342,14 +362,20 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
 
   const int64_t units = count_items(
       p.batch, [&](int b) { return absorbed_span(p, b); },
-      [&](const SeqSpan& q) { return (int64_t)row_groups(p, q, GROUP) * key_tiles(q); });
+      [&](const SeqSpan& q) { return (int64_t)row_groups(p, q, GROUP) * group_units(q); });
   const int64_t shares = units < p.shares ? units : p.shares;
   // workgroups go to the 8 XCDs by blockIdx % 8: a pair's two are 8 apart
   const int member = PAIR == 2 ? (int)(blockIdx.x / 8 % 2) : 0;
   const int64_t g = PAIR == 2 ? blockIdx.x / 16 * 8 + blockIdx.x % 8 : blockIdx.x;
   if (g >= shares) {
-    if (member == 0 && g < p.shares && threadIdx.x == 0) p.joints[g].valid = 0;
+    if (!p.by_group && member == 0 && g < p.shares && threadIdx.x == 0) p.joints[g].valid = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.groups = 0;  // no units at all
     return;
+  }
+  if (blockIdx.x == 0 && p.by_group) {
+    const int64_t n = count_items(
+        p.batch, [&](int b) { return absorbed_span(p, b); }, [&](const SeqSpan& q) { return (int64_t)row_groups(p, q, GROUP); });
+    if (threadIdx.x == 0) *p.groups = (int)n;
   }
   int64_t u = share_begin(units, g, shares);
   int left = share_size(units, g, shares);
@@ -366,15 +392,21 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
     // of a share's segments only the first can start inside a group's tiles and
     // only the last can end inside them: two partial slots a share
     const int64_t slot = 2 * g + (sg.t_begin == 0 ? 1 : 0);
-    if (!whole && sg.t_begin == 0) {
-      joint = true;
+    u += sg.units;
+    left -= sg.units;
+    if (sg.t_begin == sg.t_end) continue;  // the group's tiles begin in the next share
+    if (sg.t_begin == 0 && (a.by_group || !whole)) {
+      joint = joint || !whole;
+      int64_t at = g;
+      if (a.by_group)
+        at = sg.row0 / GROUP + count_items(
+                                   sg.b, [&](int b) { return absorbed_span(a, b); },
+                                   [&](const SeqSpan& q) { return (int64_t)row_groups(a, q, GROUP); });
       if (member == 0 && wave == 0 && lane_now() == 0) {
-        const int64_t last = share_of(opaque_uniform(units), u + sg.tiles - 1, shares);
-        a.joints[g] = Joint{seq.q0, rows, sg.row0, (int)last, 1};
+        const int64_t last = share_of(opaque_uniform(units), u - sg.units + sg.ahead, shares);
+        a.joints[at] = Joint{seq.q0, rows, sg.row0, (int)g, (int)last, whole ? 0 : 1};
       }
     }
-    u += sg.t_end - sg.t_begin;
-    left -= sg.t_end - sg.t_begin;
     if (PAIR == 2 && row0 >= rows) continue;  // the group's rows end with the other workgroup
     // query token and head of row `at` of the workgroup (rows past the last repeat it and are not stored)
     auto my_row = [&](int at, int& i, int& h) {
@@ -387,7 +419,7 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
     const int lim_min = absorbed_limit(seq, row0 / a.heads);
 
     Stager<R, P, F8> st;
-    st.begin(p, seq, sg.b, wave);
+    st.begin(p, seq, sg.b, wave, member);
     const bool any = seq.len > 0;
     if (any) st.fetch(p, sg.t_begin);
     lds_only_barrier();  // the last segment's accesses to LDS have ended
@@ -457,11 +489,13 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
                                                     ((ln % 8) ^ (uint32_t)swz_rope<false>(row)) * 16) = qp[k];
         }
       }
+      // Q's loads came first: its fragments are read while the keys are on their way
       if (any) {
-        st.finish(lds, lds + SCL);
-        if (sg.t_begin + 1 < sg.t_end) st.fetch(p, sg.t_begin + 1);
+        wait_vm<16 + (P > 0 ? T::RLOADS : 0) + (F8 ? 1 : 0)>();
+        lds_only_barrier();
+      } else {
+        loads_barrier();
       }
-      loads_barrier();
       const int ql_ = lane_now(), qq = ql_ / 16, qc = ql_ % 16;
 #pragma unroll
       for (int r = 0; r < MT; ++r)
@@ -472,6 +506,10 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
           qf[r][ks] = lds_v8bf(lds + QOFF + (ks < RS ? (16 * r + qc) * 2 * R + ((unit ^ swz_key<false>(qc)) * 16)
                                                      : ROWS * 2 * R + (16 * r + qc) * 128 + ((unit ^ swz_rope<false>(qc)) * 16)));
         }
+      if (any) {
+        st.finish(lds, lds + SCL);
+        if (sg.t_begin + 1 < sg.t_end) st.fetch(p, sg.t_begin + 1);
+      }
     }
     float m[MT], l[MT];  // the rows' reference points, their sums over this lane's keys
     v4f o[MT][DT];
@@ -501,22 +539,26 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
       const int kra = T::ROPE + krow * T::RROW + ((tq ^ swz_rope<F8>(krow)) * 16);
       // One 16-byte read of K a step (an 8-bit row's serves two MFMAs), AHEAD
       // steps before its MFMAs; the next tile's loads go between them.
-      constexpr int STEPS = F8 ? KS / 2 : KS, AHEAD = MT == 4 ? 3 : 4, RING = AHEAD + 1;
+      constexpr int STEPS = F8 ? KS / 2 : KS, AHEAD = MT < 4 ? 4 : F8 ? 2 : 3, RING = AHEAD + 1;
       auto k_at = [&](int st_) {
         if constexpr (F8) return st_ < RS / 2 ? (ka ^ ((st_ & 1) << 6)) + (st_ >> 1) * 128 : kra;
         return st_ < RS ? (ka ^ ((st_ & 3) << 6)) + (st_ >> 2) * 256 : kra ^ ((st_ - RS) << 6);
       };
       v4f s[MT];
-      {
+      // with and without the next tile's loads, as straight-line code each: a branch
+      // around every load costs a wave 30 clocks
+      auto scores = [&](auto loads_) {
+        constexpr bool LOADS = decltype(loads_)::value;
         v4i kf[RING];
 #pragma unroll
         for (int i = 0; i < AHEAD && i < STEPS; ++i) kf[i] = lds_v4i(kb + k_at(i));
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
           if (i + AHEAD < STEPS) kf[(i + AHEAD) % RING] = lds_v4i(kb + k_at(i + AHEAD));
-          #pragma unroll
-          for (int k = i * 16 / STEPS; k < (i + 1) * 16 / STEPS; ++k)
-            if (more) st.load(next, k);
+                    if constexpr (LOADS) {
+#pragma unroll
+            for (int k = i * 16 / STEPS; k < (i + 1) * 16 / STEPS; ++k) st.load(next, k);
+          }
 
           const v4i w = kf[i % RING];
           auto products = [&](auto ks_, const v8bf& a) {
@@ -538,7 +580,11 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
             }
           });
         }
-      }
+      };
+      if (more)
+        scores(std::true_type{});
+      else
+        scores(std::false_type{});
       if constexpr (MT > 1) qk_done<MT>(s);
       if (more) st.parts(p);  // not before: their registers are K's until here
       __builtin_amdgcn_sched_barrier(0);
@@ -706,26 +752,94 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
         *(uint2*)(orow + 16 * t) = make_uint2(pack_bf16(o[r][t][0] * inv, o[r][t][1] * inv), pack_bf16(o[r][t][2] * inv, o[r][t][3] * inv));
     }
   }
-  if (!joint && member == 0 && wave == 0 && lane_now() == 0) p.joints[g].valid = 0;
+  if (!p.by_group && !joint && member == 0 && wave == 0 && lane_now() == 0) p.joints[g].valid = 0;
 }
 
 // ---- joining the partial results ------------------------------------------------
 //
-// One workgroup a strip of 16 rows and PIECES of its 1 KB pieces (64 lanes x 4
-// values: 16 of the latent dimension for each row); its waves split the
-// partials, each keeping a running maximum and sum, and meet in LDS.
-template <int R, int ROWS, int PIECES>
-__global__ __launch_bounds__(256) void absorbed_combine_kernel(const Absorbed p) {
-  constexpr int STRIPS = ROWS / 16, ALL = R / 16;
-  __shared__ float sm[4][64], sl[4][64];
-  __shared__ float4 so[4][PIECES][64];
+// The joint of a strip of 16 rows (workgroup `item` of STRIPS a group), or none.
+template <int STRIPS>
+__device__ __forceinline__ bool find_joint(const Absorbed& p, int64_t item, Joint* j, int* strip) {
+  *strip = (int)(item % STRIPS);
+  const int64_t at = item / STRIPS;
+  if (p.by_group && at >= *p.groups) return false;
+  *j = p.joints[at];
+  return j->valid && j->row0 + *strip * 16 < j->rows;
+}
+
+// Partial results of many shares: each of the 16 waves takes four at a time, 16
+// lanes for the 16 rows' 4 values of one latent piece, so that a strip's
+// partials (R / 4 workgroups of them) spread over many CUs: a CU takes some 10
+// bytes a clock that its L2 does not have (256 shares of one sequence in 32
+// workgroups took 23 us, in 128 6).
+template <int R, int ROWS>
+__global__ __launch_bounds__(1024) void absorbed_combine_many_kernel(const Absorbed p) {
+  constexpr int STRIPS = ROWS / 16, ALL = R / 16, WAVES = 16;
+  __shared__ float sm[WAVES][16], sl[WAVES][16];
+  __shared__ float4 so[WAVES][16];
+  Joint j;
+  int strip;
+  if (!find_joint<STRIPS>(p, blockIdx.x, &j, &strip)) return;
   const int lane = (int)threadIdx.x % kWave, wave = (int)threadIdx.x / kWave;
-  const int strip = (int)(blockIdx.x % STRIPS);
-  const int64_t g0 = blockIdx.x / STRIPS;
-  const Joint j = p.joints[g0];
+  const int row = lane % 16, piece = (int)blockIdx.y / 4, q = (int)blockIdx.y % 4;
+  float m = -INFINITY, l = 0.0f;
+  float4 acc = make_float4(0, 0, 0, 0);
+  auto take = [&](float m2, float l2, const float4& v) {
+    const float mn = fmaxf(m, m2);
+    const float a = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    const float w = l2 == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m2 - mn);
+    m = mn;
+    l = l * a + l2 * w;
+    acc.x = acc.x * a + v.x * w;
+    acc.y = acc.y * a + v.y * w;
+    acc.z = acc.z * a + v.z * w;
+    acc.w = acc.w * a + v.w * w;
+  };
+#pragma unroll 4
+  for (int64_t g = j.first + 4 * wave + lane / 16; g <= j.last; g += 4 * WAVES) {
+    const int64_t slot = 2 * g + (g == j.first ? 1 : 0);
+    const float ls = p.part_lse[slot * ROWS + strip * 16 + row];
+    const float4 v = ((const float4*)p.part_o)[((slot * STRIPS + strip) * ALL + piece) * 64 + q * 16 + row];
+    take(ls, ls == -INFINITY ? 0.0f : 1.0f, v);
+  }
+#pragma unroll
+  for (int o = 16; o <= 32; o <<= 1) {
+    const float4 v = make_float4(__shfl_xor(acc.x, o), __shfl_xor(acc.y, o), __shfl_xor(acc.z, o), __shfl_xor(acc.w, o));
+    const float m2 = __shfl_xor(m, o), l2 = __shfl_xor(l, o);
+    take(m2, l2, v);
+  }
+  if (lane < 16) {
+    sm[wave][row] = m;
+    sl[wave][row] = l;
+    so[wave][row] = acc;
+  }
+  __syncthreads();
+  if (wave != 0 || lane >= 16) return;
+  for (int w = 1; w < WAVES; ++w) take(sm[w][row], sl[w][row], so[w][row]);
+  const int at = j.row0 + strip * 16 + row;
+  if (at >= j.rows) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int64_t token = j.q0 + at / p.heads;
+  const int h = at % p.heads;
+  if (p.lse && blockIdx.y == 0) p.lse[token * p.heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+  *(uint2*)(p.out + token * p.ot + h * p.oh + 16 * piece + 4 * q) =
+      make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+}
+
+// Of a few shares: one workgroup a strip of 16 rows and 4 of its 1 KB pieces (64
+// lanes x 4 values: 16 of the latent dimension for each row); its waves split
+// the partials, each keeping a running maximum and sum, and meet in LDS.
+template <int R, int ROWS>
+__global__ __launch_bounds__(256) void absorbed_combine_kernel(const Absorbed p) {
+  constexpr int STRIPS = ROWS / 16, ALL = R / 16, PIECES = 4, WAVES = 4;
+  __shared__ float sm[WAVES][64], sl[WAVES][64];
+  __shared__ float4 so[WAVES][PIECES][64];
+  Joint j;
+  int strip;
+  if (!find_joint<STRIPS>(p, blockIdx.x, &j, &strip)) return;
+  const int lane = (int)threadIdx.x % kWave, wave = (int)threadIdx.x / kWave;
   const int row = j.row0 + strip * 16 + lane % 16;
-  if (!j.valid || j.row0 + strip * 16 >= j.rows) return;
-  const int64_t g1 = j.last;
+  const int64_t g0 = j.first, g1 = j.last;
   const int piece0 = (int)blockIdx.y * PIECES;
 
   float m = -INFINITY, l = 0.0f;
@@ -733,7 +847,7 @@ __global__ __launch_bounds__(256) void absorbed_combine_kernel(const Absorbed p)
 #pragma unroll
   for (int k = 0; k < PIECES; ++k) acc[k] = make_float4(0, 0, 0, 0);
 #pragma unroll 2
-  for (int64_t g = g0 + wave; g <= g1; g += 4) {
+  for (int64_t g = g0 + wave; g <= g1; g += WAVES) {
     const int64_t slot = 2 * g + (g == g0 ? 1 : 0);
     const float ls = p.part_lse[slot * ROWS + strip * 16 + lane % 16];
     const float4* po = (const float4*)p.part_o + ((slot * STRIPS + strip) * ALL + piece0) * 64 + lane;
@@ -758,11 +872,11 @@ __global__ __launch_bounds__(256) void absorbed_combine_kernel(const Absorbed p)
 #pragma unroll
   for (int k = 0; k < PIECES; ++k) so[wave][k][lane] = acc[k];
   __syncthreads();
-  float top = -INFINITY, total = 0.0f, w[4];
+  float top = -INFINITY, total = 0.0f, w[WAVES];
 #pragma unroll
-  for (int v = 0; v < 4; ++v) top = fmaxf(top, sm[v][lane]);
+  for (int v = 0; v < WAVES; ++v) top = fmaxf(top, sm[v][lane]);
 #pragma unroll
-  for (int v = 0; v < 4; ++v) {
+  for (int v = 0; v < WAVES; ++v) {
     // a wave that saw no key has l == 0 and nothing in its sums
     w[v] = sl[v][lane] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(sm[v][lane] - top);
     total += w[v] * sl[v][lane];
@@ -774,10 +888,10 @@ __global__ __launch_bounds__(256) void absorbed_combine_kernel(const Absorbed p)
   if (p.lse && piece0 == 0 && wave == 0 && lane < 16)
     p.lse[token * p.heads + h] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
   uint16_t* orow = p.out + token * p.ot + h * p.oh + 4 * (lane / 16);
-  for (int k = wave; k < PIECES; k += 4) {
+  for (int k = wave; k < PIECES; k += WAVES) {
     float4 r = make_float4(0, 0, 0, 0);
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
+    for (int v = 0; v < WAVES; ++v) {
       const float4 x = so[v][k][lane];
       r.x += w[v] * x.x;
       r.y += w[v] * x.y;
@@ -794,6 +908,7 @@ struct AbsPlan {
   int rows;        // of a row group: 16, 32, 64, or 128 in two workgroups
   int64_t groups;  // upper bound of the batch's row groups
   int64_t shares;  // the units are divided into
+  bool by_group;
   size_t joint_bytes, lse_bytes, bytes;
 };
 
@@ -808,9 +923,10 @@ AbsPlan absorbed_plan(const fcmoe_absorbed_args* a) {
     (void)hipGetLastError();
   // One workgroup a CU (two LDS buffers fill it); 8-bit rows of 16 leave room for two.
   const int64_t slots = pl.rows == 128 ? cus / 2 : (int64_t)cus * (a->cache.e4m3 && pl.rows == 16 ? 2 : 1);
-  const int64_t most = pl.groups * (a->table_width > 0 ? ceil_div(a->table_width * a->cache.page_size, kAbsKeys) : 1);
+  const int64_t most = pl.groups * ((a->table_width > 0 ? ceil_div(a->table_width * a->cache.page_size, kAbsKeys) : 1) + kGroupCost);
   pl.shares = most < slots ? (most > 0 ? most : 1) : slots;
-  pl.joint_bytes = (size_t)round_up(pl.shares * (int64_t)sizeof(Joint), 256);
+  pl.by_group = pl.groups <= pl.shares;
+  pl.joint_bytes = 256 + (size_t)round_up((pl.by_group ? pl.groups : pl.shares) * (int64_t)sizeof(Joint), 256);
   pl.lse_bytes = (size_t)round_up(2 * pl.shares * pl.rows * 4, 256);
   pl.bytes = pl.joint_bytes + pl.lse_bytes + (size_t)(2 * pl.shares) * (size_t)pl.rows * (size_t)a->cache.latent_dim * 4;
   return pl;
@@ -831,18 +947,23 @@ void absorbed_launch(const Absorbed& p, const AbsPlan& pl, hipStream_t stream) {
 
 template <int R>
 void combine_launch(const Absorbed& p, const AbsPlan& pl, hipStream_t stream) {
-  const dim3 b(256);
-  const unsigned g = (unsigned)pl.shares;
+  auto go = [&](auto rows_) {
+    constexpr int ROWS = decltype(rows_)::value;
+    const int64_t strips = (pl.by_group ? pl.groups : pl.shares) * (ROWS / 16);
+    // few strips: their partials are spread over more workgroups
+    if (strips * (R / 4) <= 4096)
+      hipLaunchKernelGGL((absorbed_combine_many_kernel<R, ROWS>), dim3((unsigned)strips, R / 4), dim3(1024), 0, stream, p);
+    else
+      hipLaunchKernelGGL((absorbed_combine_kernel<R, ROWS>), dim3((unsigned)strips, R / 64), dim3(256), 0, stream, p);
+  };
   if (pl.rows == 128)
-    hipLaunchKernelGGL((absorbed_combine_kernel<R, 128, 4>), dim3(g * 8, R / 64), b, 0, stream, p);
+    go(std::integral_constant<int, 128>{});
   else if (pl.rows == 64)
-    hipLaunchKernelGGL((absorbed_combine_kernel<R, 64, 4>), dim3(g * 4, R / 64), b, 0, stream, p);
+    go(std::integral_constant<int, 64>{});
   else if (pl.rows == 32)
-    hipLaunchKernelGGL((absorbed_combine_kernel<R, 32, 4>), dim3(g * 2, R / 64), b, 0, stream, p);
-  else if (pl.groups >= 64)
-    hipLaunchKernelGGL((absorbed_combine_kernel<R, 16, 4>), dim3(g, R / 64), b, 0, stream, p);
+    go(std::integral_constant<int, 32>{});
   else
-    hipLaunchKernelGGL((absorbed_combine_kernel<R, 16, 1>), dim3(g, R / 16), b, 0, stream, p);
+    go(std::integral_constant<int, 16>{});
 }
 
 int check_absorbed(const fcmoe_absorbed_args* a) {
@@ -853,7 +974,7 @@ int check_absorbed(const fcmoe_absorbed_args* a) {
       a->page_table_stride < 0)
     return fail(FCMOE_EINVAL, "absorbed_attention: bad shape");
   // units are counted in 32 bits a sequence
-  if (ceil_div(a->tokens * a->heads, 16) + a->batch > INT32_MAX / (ceil_div(a->table_width * a->cache.page_size, kAbsKeys) + 1))
+  if (ceil_div(a->tokens * a->heads, 16) + a->batch > INT32_MAX / (ceil_div(a->table_width * a->cache.page_size, kAbsKeys) + kGroupCost + 1))
     return fail(FCMOE_EINVAL, "absorbed_attention: too many rows for a page table of this reach");
   if (!a->query_starts && a->tokens != a->batch)
     return fail(FCMOE_EINVAL, "absorbed_attention: without query_starts there is one token a sequence");
@@ -895,7 +1016,9 @@ extern "C" int fcmoe_absorbed_attention(const fcmoe_absorbed_args* a, hipStream_
   p.tokens = a->tokens, p.batch = (int)a->batch, p.heads = (int)a->heads;
   p.scale = a->scale;
   p.out = a->out, p.ot = a->out_token_stride, p.oh = a->out_head_stride, p.lse = a->lse;
-  p.joints = (Joint*)a->workspace;
+  p.groups = (int*)a->workspace;
+  p.joints = (Joint*)((char*)a->workspace + 256);
+  p.by_group = pl.by_group;
   p.part_lse = (float*)((char*)a->workspace + pl.joint_bytes);
   p.part_o = (float*)((char*)a->workspace + pl.joint_bytes + pl.lse_bytes);
   p.shares = (int)pl.shares;
