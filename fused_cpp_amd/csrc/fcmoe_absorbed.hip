@@ -30,7 +30,6 @@ namespace fcmoe {
 namespace {
 
 constexpr int kAbsKeys = 64;  // keys of a tile
-constexpr int kBufWord3 = 0x00020000;  // raw buffer resource word 3 for gfx9: 32-bit data format, no swizzle
 
 // A row group whose tiles end up with several shares: left by the share that
 // has its first tile for the launch that joins the partial results. Kept by

@@ -29,6 +29,7 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 
+constexpr int kBufWord3 = 0x00020000;  // raw buffer resource word 3 for gfx9: 32-bit data format, no swizzle
 constexpr float kE4M3Max = 448.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -63,10 +64,10 @@ __device__ __forceinline__ v8bf widen_e4m3(v2i u) {
 // takes a block of 4 rows x 16 values (row j at the addresses of lanes 4 j ..
 // 4 j + 3, 8 bytes each) and gives lane i column i; ds_read_b64_tr_b8 takes
 // 8 rows x 16 bytes (row j at lanes 2 j, 2 j + 1) and gives lane i column i.
-__device__ __forceinline__ v4s read_tr16(const lds_u8* p) {
+__device__ __forceinline__ v4s read_tr16(const lds_u8* __restrict__ p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)p);
 }
-__device__ __forceinline__ v2i read_tr8(const lds_u8* p) {
+__device__ __forceinline__ v2i read_tr8(const lds_u8* __restrict__ p) {
   return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)p);
 }
 __device__ __forceinline__ v8bf join_tr16(v4s lo, v4s hi) {
@@ -75,10 +76,14 @@ __device__ __forceinline__ v8bf join_tr16(v4s lo, v4s hi) {
 }
 
 // 16 bytes a lane from memory straight to LDS: lane l's land at dst + 16 l
-// (dst the same in all lanes). Counts in vmcnt.
+// (dst the same in all lanes). Counts in vmcnt. The second form reads a buffer
+// at a byte offset, zeros past its end.
 __device__ __forceinline__ void load_lds16(const void* src, lds_u8* dst) {
   __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)src,
                                    (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+__device__ __forceinline__ void load_lds16(const __amdgpu_buffer_rsrc_t src, lds_u8* dst, uint32_t offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)dst, 16, offset, 0, 0, 0);
 }
 
 template <int N>

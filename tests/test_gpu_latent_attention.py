@@ -590,6 +590,86 @@ def test_expanded_keeps_to_its_sequence(gpu):
     assert torch.equal(cut, want)
 
 
+# An average of more than 128 new tokens and 1024 keys: blocks of 256 query rows.
+WIDE_NEW, WIDE_LENS = [0, 300, 1, 0, 700, 257, 64], [9, 3000, 2500, 0, 700, 257, 2600]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("N,P", HEADS)
+@pytest.mark.parametrize("H", [1, 3])
+def test_expanded_long_prompts(gpu, H, N, P, causal):
+    q, kv, kr = _expanded_inputs(H, WIDE_NEW, WIDE_LENS, H, N, P)
+    out, lse = _check_expanded(q, kv, kr, _bounds(WIDE_NEW), _bounds(WIDE_LENS), 0.08, causal)
+    again = _la().expanded_attention(q, kv, kr, _i32(_bounds(WIDE_NEW)), kv_starts=_i32(_bounds(WIDE_LENS)), scale=0.08,
+                                     causal=causal, return_lse=True)
+    assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+
+
+@pytest.mark.parametrize("new,lens", [([2200], [2140]),  # the first 60 query tokens see no key
+                                      ([129], [40000]), ([1030, 250], [5000, 250]), ([2049] * 3, [2049] * 3)])
+def test_expanded_long_prompt_blocks(gpu, new, lens):
+    """Rows that see nothing, a key axis shared by workgroups, and more row blocks than CUs."""
+    H = 12 if len(new) == 3 else 2
+    q, kv, kr = _expanded_inputs(9, new, lens, H, 128, 64)
+    _check_expanded(q, kv, kr, _bounds(new), _bounds(lens), 0.08, True)
+
+
+@pytest.mark.parametrize("N,P", HEADS)
+@pytest.mark.parametrize("sign", [1, -1])
+def test_expanded_long_prompt_growing_scores(gpu, N, P, sign):
+    """Scores that climb by 40 every 16 keys, past what a first tile's maximum can hold, and that fall as fast."""
+    new = [2300]
+    q, kv, kr = _expanded_inputs(10, new, new, 2, N, P, std=0.5)
+    q[..., 0] = 1.0
+    kv[:, :, 0] = ((torch.arange(2300, device="cuda") // 16) * 40.0 * sign).to(BF16)[:, None]
+    _check_expanded(q, kv, kr, [0, 2300], [0, 2300], 1.0, True)
+
+
+def test_expanded_long_prompt_neighbours(gpu):
+    """Keys outside a sequence may be anything, in memory and left over on the chip."""
+    la = _la()
+    new = [2150, 40]
+    q, kv, kr = _expanded_inputs(11, new, new, 4, 128, 64)
+    want, _ = _check_expanded(q[:2150], kv[:2150], kr[:2150], [0, 2150], [0, 2150], 0.08, True)
+    bad_kv, bad_kr = torch.full_like(kv, math.nan), torch.full_like(kr, math.inf)
+    la.expanded_attention(q[:2150], bad_kv[:2150], bad_kr[:2150], _i32([0, 2150]), scale=0.08)
+    kv2, kr2 = bad_kv.clone(), bad_kr.clone()
+    kv2[:2150], kr2[:2150] = kv[:2150], kr[:2150]
+    assert torch.equal(la.expanded_attention(q[:2150], kv2, kr2, _i32([0, 2150]), scale=0.08), want)
+    # starts outside the tensors are cut to them; a caller's rows outside the sequences stay
+    pad = torch.cat([q[:1], q[:2150], q[:3]])
+    kept = torch.full((2154, 4, 128), 5.0, dtype=BF16, device="cuda")
+    la.expanded_attention(pad, kv[:2150], kr[:2150], _i32([1, 2151]), kv_starts=_i32([-3, 9999]), scale=0.08, out=kept)
+    assert torch.equal(kept[1:2151], want) and bool((kept[0] == 5).all()) and bool((kept[2151:] == 5).all())
+    got, lse = la.expanded_attention(pad, kv[:2150], kr[:2150], _i32([1, 2151]), kv_starts=_i32([0, 2150]), scale=0.08,
+                                     return_lse=True)
+    assert torch.equal(got[1:2151], want) and bool((got[0] == 0).all()) and bool((got[2151:] == 0).all())
+    assert bool((lse[0] == -math.inf).all()) and bool((lse[2151:] == -math.inf).all())
+
+
+def test_expanded_long_prompt_strides(gpu):
+    la = _la()
+    q, kv, kr = _expanded_inputs(12, [2100], [2100], 4, 128, 64)
+    st = _i32([0, 2100])
+    want = la.expanded_attention(q, kv, kr, st, scale=0.08)
+    heads_first = lambda x: x.transpose(0, 1).contiguous().transpose(0, 1)  # noqa: E731
+    rows = torch.zeros((2100, 576), dtype=BF16, device="cuda")
+    rows[:, 512:] = kr
+    assert torch.equal(la.expanded_attention(heads_first(q), heads_first(kv), rows[:, 512:], st, scale=0.08), want)
+    one = kv[:, :1].expand(2100, 4, 256)
+    assert torch.equal(la.expanded_attention(q, one, kr, st, scale=0.08),
+                       la.expanded_attention(q, one.contiguous(), kr, st, scale=0.08))
+
+
+@pytest.mark.parametrize("rows", [5, 150])
+def test_expanded_many_sequences(gpu, rows):
+    """More sequences than a wave has lanes, empty ones among them."""
+    new = [(rows if b % 3 else 0) for b in range(150)] + [1]
+    lens = [n + (40 if rows == 5 else 1500 * (b % 50 == 1)) for b, n in enumerate(new)]
+    q, kv, kr = _expanded_inputs(13, new, lens, 1, 64, 0)
+    _check_expanded(q, kv, kr, _bounds(new), _bounds(lens), 0.1, True)
+
+
 def test_expanded_rows_past_32_bit_offsets(gpu):
     S, H = 70000, 128
     kv = torch.empty((S, H, 256), dtype=BF16, device="cuda")
