@@ -66,6 +66,7 @@ struct Absorbed {
   int by_group;
   int shares;
   int page_shift;  // log2 of a page size that is a power of two, else -1
+  int whole;       // pages hold multiples of 16 keys
   int zero_tail;
 };
 
@@ -175,7 +176,10 @@ typedef __attribute__((address_space(1))) v4i global_v4i;  // an address from in
 // in scalar registers; they are buffer loads, because after a global load to
 // LDS the compiler waits for all of a wave's LDS reads wherever it needs one.
 // The key parts and scales (rows too short for a load each) pass through
-// registers.
+// registers. Where a wave's 16 keys lie in one page and all exist (pages of a
+// multiple of 16 keys, tiles before the last), one address serves them all, a
+// load brings 1 KB of them whatever the rows' length, and the key parts and
+// scales go straight to LDS too: 128 heads, 64 sequences 161 us -> 148.
 template <int R, int P, bool F8>
 struct Stager {
   using T = Tile<R, P, F8>;
@@ -186,6 +190,14 @@ struct Stager {
   uint64_t lat;  // the tile being brought in
   v4i part[P > 0 ? T::RLOADS : 1];
   float scale;
+  // a tile whose 64 keys all exist, in pages of multiples of 16: the wave's 16
+  // keys are neighbours in memory, first latent row, key part and scale here
+  uint64_t wl, wr, ws;
+  uint32_t step, rstep;  // bytes between rows
+  bool whole;
+  static constexpr int KPL = 1024 / T::LROW;       // keys a load of 1 KB brings
+  static constexpr int RKPL = P > 0 ? 1024 / T::RROW : 1;
+  static constexpr int WLOADS = 16 / KPL, WRLOADS = P > 0 ? 16 / RKPL : 0;
 
   __device__ __forceinline__ void begin(const Absorbed& p, const SeqSpan& s, int b, int w, int member) {
     wave = w;
@@ -196,9 +208,15 @@ struct Stager {
   __device__ __forceinline__ void fetch(const Absorbed& p, int tile) {
     int key = tile * kAbsKeys + 16 * wave + lane_now() % 16;
     key = key < last_key ? key : last_key;  // keys past the length re-read its last one; their scores are masked
-    const uint32_t size = (uint32_t)p.c.page_size;
-    const uint32_t page = p.page_shift >= 0 ? (uint32_t)key >> p.page_shift : (uint32_t)key / (uint32_t)opaque_uniform((int)size);
-    in = key - (int)(page * size);
+    uint32_t page;
+    if (opaque_uniform(p.page_shift) >= 0) {
+      page = (uint32_t)key >> p.page_shift;
+      in = key - (int)(page << p.page_shift);
+    } else {
+      const uint32_t size = (uint32_t)opaque_uniform((int)p.c.page_size);
+      page = (uint32_t)key / size;
+      in = key - (int)(page * size);
+    }
     id = table[page];
   }
   // The fetched tile's latent addresses.
@@ -207,6 +225,47 @@ struct Stager {
     if (bad) id = 0;
     if (__any(bad)) *(lds_i32*)bad_flag = 1;  // every lane writes the same
     lat = (uint64_t)p.c.latent + (id * p.c.latent_page_stride + in * p.c.latent_row_stride) * T::ELEM;
+  }
+  __device__ __forceinline__ void start_whole(const Absorbed& p, lds_u8* bad_flag) {
+    uint32_t page = (uint32_t)uniform(id);
+    const uint32_t row = (uint32_t)uniform(in);
+    if (page >= (uint32_t)p.c.pages) {
+      page = 0;
+      *(lds_i32*)bad_flag = 1;
+    }
+    // pages of less than 4 GB: products of 32 bits by 32
+    step = (uint32_t)(p.c.latent_row_stride * T::ELEM);
+    wl = (uint64_t)p.c.latent + (uint64_t)page * (uint32_t)(p.c.latent_page_stride * T::ELEM) + row * step;
+    if constexpr (P > 0) {
+      rstep = (uint32_t)(p.c.rope_row_stride * T::ELEM);
+      wr = (uint64_t)p.c.rope + (uint64_t)page * (uint32_t)(p.c.rope_page_stride * T::ELEM) + row * rstep;
+    }
+    if constexpr (F8) ws = (uint64_t)p.c.scale + (uint64_t)page * (uint32_t)(p.c.scale_page_stride * 4) + row * 4;
+    wl = (uint64_t)opaque_uniform((int64_t)wl);  // or the compiler merges its store with that of `lat`, through memory
+  }
+  // Of such a tile: load u of WLOADS + WRLOADS (latent rows, then key parts).
+  template <int u>
+  static __device__ __forceinline__ void load_whole(lds_u8* dst, uint64_t wl, uint64_t wr, uint32_t step, uint32_t rstep,
+                                                    int lane16, int lane_row, int wave, int turn) {
+    if constexpr (u < WLOADS) {
+      const int half = (KPL * u) & 8 ? turn ^ 8 : turn;  // the first key of the eight that the load is in
+      load_lds16(rows_at(wl, 15 * step + T::LROW), dst + (16 * wave + half + KPL * u % 8) * T::LROW,
+                 (uint32_t)((lane16 ^ ((swz_key<F8>(KPL * u % 8) * 16) ^ (F8 ? half / 2 : half) * 16)) + lane_row),
+                 step * (uint32_t)(half + KPL * u % 8));
+    } else if constexpr (P > 0) {
+      const int ln = lane_now(), k = ln / T::RUNITS;
+      load_lds16(rows_at(wr, 15 * rstep + T::RROW), dst + T::ROPE + (16 * wave + RKPL * (u - WLOADS)) * T::RROW,
+                 (uint32_t)(k * (int)rstep + ((ln % T::RUNITS) ^ swz_rope<F8>(k)) * 16), rstep * (uint32_t)(RKPL * (u - WLOADS)));
+    }
+  }
+  __device__ __forceinline__ void scales_whole(lds_u8* scl) const {
+    if constexpr (F8) {
+      const int ln = lane_now();
+      if (ln < 16) load_lds4(rows_at(ws, 64), scl + 64 * wave, (uint32_t)ln * 4);
+    }
+  }
+  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(uint64_t base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)bytes, kBufWord3);
   }
   // Its key parts and scales on their way to registers.
   __device__ __forceinline__ void parts(const Absorbed& p) {
@@ -280,7 +339,8 @@ __device__ __forceinline__ v4f lds_v4f(const lds_u8* p) { return *(const __attri
 // take all of a SIMD's 512 for its one wave. Half of those are accumulation
 // registers, which MFMAs can read as operands; Q lies there, and its MFMAs are
 // written out, because the compiler would copy each fragment to an ordinary
-// register first (a tile of 64 rows took 10000 clocks, now 6900). With eight
+// register first (a tile of 64 rows took 10000 clocks, with that 6900, now
+// 6300; its products alone 2200). With eight
 // waves instead, Q leaves no registers to read K fragments ahead with (9200).
 //
 // PAIR: the rows of a sequence fill two workgroups (65 rows and more); these
@@ -324,9 +384,9 @@ __device__ __forceinline__ void mfma_qk(v4f& acc, const v8bf& k, const v8bf& q) 
 template <int N>
 __device__ __forceinline__ void qk_done(v4f* s) {
   if constexpr (N == 2)
-    asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1]));
+    asm volatile("s_nop 11" : "+v"(s[0]), "+v"(s[1]));
   else
-    asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3]));
+    asm volatile("s_nop 11" : "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3]));
 }
 
 // The kernel's arguments, read anew from the kernarg segment: what only the
@@ -378,7 +438,7 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
   }
   int64_t u = share_begin(units, g, shares);
   int left = share_size(units, g, shares);
-  bool joint = false;  // a joint of this share was written
+  int joint = 0;  // a joint of this share was written
   const float c2 = uniform(p.scale * kLog2e);
 
   while (left > 0) {
@@ -395,7 +455,7 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
     left -= sg.units;
     if (sg.t_begin == sg.t_end) continue;  // the group's tiles begin in the next share
     if (sg.t_begin == 0 && (a.by_group || !whole)) {
-      joint = joint || !whole;
+      joint = uniform(joint | (whole ? 0 : 1));
       int64_t at = g;
       if (a.by_group)
         at = sg.row0 / GROUP + count_items(
@@ -520,11 +580,23 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
       for (int t = 0; t < DT; ++t) o[r][t] = v4f{0, 0, 0, 0};
     }
 
+    // what the loads of a tile need, formed at the end of the tile before the one they go among
+    auto start = [&](int tile) {
+      st.whole = false;
+      if (tile >= sg.t_end) return;
+      const Absorbed b = args_now();
+      st.whole = b.whole && (tile + 1) * kAbsKeys <= seq.len;
+      if (st.whole)
+        st.start_whole(b, lds + FLAGS + 8);
+      else
+        st.start(b, lds + FLAGS + 8);
+    };
+    if (any) start(sg.t_begin + 1);
     for (int tile = sg.t_begin; any && tile < sg.t_end; ++tile) {
       const int buf = (tile - sg.t_begin) & 1;
       const bool more = tile + 1 < sg.t_end;
       loads_barrier();  // the tile has landed; everyone is done with the other buffer
-      if (more) st.start(p, lds + FLAGS + 8);
+      const bool whole = st.whole;  // the next tile
       const lds_u8* kb = lds + buf * T::BYTES;
       lds_u8* next = lds + (buf ^ 1) * T::BYTES;
       // What depends on the lane is formed here, in each tile, and addresses
@@ -537,28 +609,36 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
       const int ka = krow * T::LROW + ((tq ^ swz_key<F8>(krow)) * 16);
       const int kra = T::ROPE + krow * T::RROW + ((tq ^ swz_rope<F8>(krow)) * 16);
       // One 16-byte read of K a step (an 8-bit row's serves two MFMAs), AHEAD
-      // steps before its MFMAs; the next tile's loads go between them.
-      constexpr int STEPS = F8 ? KS / 2 : KS, AHEAD = MT < 4 ? 4 : F8 ? 2 : 3, RING = AHEAD + 1;
+      // steps before its MFMAs (as many as there are registers for); the next tile's loads go between them.
+      constexpr int STEPS = F8 ? KS / 2 : KS, AHEAD = MT < 4 ? 4 : F8 ? PAIR : 3, RING = AHEAD + 1;
       auto k_at = [&](int st_) {
         if constexpr (F8) return st_ < RS / 2 ? (ka ^ ((st_ & 1) << 6)) + (st_ >> 1) * 128 : kra;
         return st_ < RS ? (ka ^ ((st_ & 3) << 6)) + (st_ >> 2) * 256 : kra ^ ((st_ - RS) << 6);
       };
       v4f s[MT];
-      // with and without the next tile's loads, as straight-line code each: a branch
-      // around every load costs a wave 30 clocks
+      // with either kind and without the next tile's loads, as straight-line code
+      // each: a branch around every load costs a wave 30 clocks
       auto scores = [&](auto loads_) {
-        constexpr bool LOADS = decltype(loads_)::value;
+        constexpr int LOADS = decltype(loads_)::value;
+        static_assert(STEPS == Stager<R, P, F8>::WLOADS + Stager<R, P, F8>::WRLOADS, "a load a step");
+        using S = Stager<R, P, F8>;
+        const uint64_t wl = st.wl, wr = st.wr;
+        const uint32_t step = st.step, rstep = st.rstep;
+        const int wave = st.wave, turn = st.turn;
+        const int part = tl / S::T::UNITS;  // of a load's keys, this lane's
+        const int lane16 = ((tl % S::T::UNITS) ^ swz_key<F8>(part)) * 16, lane_row = S::KPL > 1 ? part * (int)step : 0;
         v4i kf[RING];
 #pragma unroll
         for (int i = 0; i < AHEAD && i < STEPS; ++i) kf[i] = lds_v4i(kb + k_at(i));
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
           if (i + AHEAD < STEPS) kf[(i + AHEAD) % RING] = lds_v4i(kb + k_at(i + AHEAD));
-                    if constexpr (LOADS) {
+          if constexpr (LOADS == 1) {
 #pragma unroll
             for (int k = i * 16 / STEPS; k < (i + 1) * 16 / STEPS; ++k) st.load(next, k);
+          } else if constexpr (LOADS == 2) {
+            unroll_at<STEPS>(i, [&](auto i_) { st.template load_whole<decltype(i_)::value>(next, wl, wr, step, rstep, lane16, lane_row, wave, turn); });
           }
-
           const v4i w = kf[i % RING];
           auto products = [&](auto ks_, const v8bf& a) {
             constexpr int ks = decltype(ks_)::value;
@@ -580,12 +660,17 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
           });
         }
       };
-      if (more)
-        scores(std::true_type{});
+      if (whole)
+        scores(std::integral_constant<int, 2>{});
+      else if (more)
+        scores(std::integral_constant<int, 1>{});
       else
-        scores(std::false_type{});
+        scores(std::integral_constant<int, 0>{});
       if constexpr (MT > 1) qk_done<MT>(s);
-      if (more) st.parts(p);  // not before: their registers are K's until here
+      if (whole)
+        st.scales_whole(lds + SCL + (buf ^ 1) * 256);
+      else if (more)
+        st.parts(args_now());  // not before: their registers are K's until here
       __builtin_amdgcn_sched_barrier(0);
       // lane: row tc of each row tile, keys 16 wave + 4 tq + i
       if constexpr (F8) {
@@ -636,7 +721,43 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
       };
       weights();
       lds_only_barrier();
-      if (__builtin_amdgcn_readfirstlane(*(lds_i32*)(lds + FLAGS + 4 * buf))) {
+      const int far = *(lds_i32*)(lds + FLAGS + 4 * buf);
+      // V^T reads: this lane's place in its group's block of keys 8 vq .. 8 vq + 7;
+      // unit u0 of the wave's quarter, whose other units differ from it in address
+      // bits that neither the key nor the lane touches
+      const int vl = lane_now(), vq = vl / 16, vc = vl % 16;
+      const int vkey = F8 ? 8 * vq + vc / 2 : 8 * vq + vc / 4;
+      const int u0 = F8 ? wave * DT : 2 * wave * DT + (vc % 4) / 2;
+      const int va = vkey * T::LROW + ((u0 ^ swz_key<F8>(vkey)) * 16) + (vl & 1) * 8;
+      // V fragments are read ahead of their MFMAs (the schedule is pinned: left to
+      // itself the compiler reads each where it is used, and every d tile waits out
+      // the LDS latency)
+      constexpr int VN = 2 * DT, VAHEAD = 4, VRING = VAHEAD + 1;
+      v4s vlo[VRING], vhi[VRING];
+      v2i v8[VRING];
+      auto v_read = [&](int n) {
+        const int s2 = n / DT, t = n % DT;
+        if constexpr (F8) {
+          v8[n % VRING] = read_tr8(kb + (va ^ (t << 4)) + 32 * s2 * T::LROW);
+        } else {
+          vlo[n % VRING] = read_tr16(kb + (va ^ (t << 5)) + 32 * s2 * T::LROW);
+          vhi[n % VRING] = read_tr16(kb + (va ^ ((t << 5) | 16)) + (32 * s2 + 4) * T::LROW);  // keys + 4: swizzle bit 0
+        }
+      };
+      v8bf pf[2][MT];
+      auto p_read = [&](int s2, int r0 = 0, int r1 = MT) {
+#pragma unroll
+        for (int r = r0; r < r1; ++r) pf[s2][r] = lds_v8bf(lds + PBUF + (16 * r + vc) * PROW + (32 * s2 + 8 * vq) * 2);
+      };
+      // ahead of the decision where there are registers: S is needed until then
+      constexpr bool EARLY = MT < 4;
+      auto first_reads = [&]() {
+        p_read(0);
+#pragma unroll
+        for (int n = 0; n < VAHEAD; ++n) v_read(n);
+      };
+      if constexpr (EARLY) first_reads();
+      if (__builtin_amdgcn_readfirstlane(far)) {
         // some row's maximum has grown: exchange maxima, rescale, form P again
         const int rl = lane_now();
 #pragma unroll
@@ -661,54 +782,29 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
         }
         weights();
         lds_only_barrier();
+        if constexpr (EARLY) first_reads();  // anew: not kept through the above
       }
-      // V^T reads: this lane's place in its group's block of keys 8 vq .. 8 vq + 7;
-      // unit u0 of the wave's quarter, whose other units differ from it in address
-      // bits that neither the key nor the lane touches
-      const int vl = lane_now(), vq = vl / 16, vc = vl % 16;
-      const int vkey = F8 ? 8 * vq + vc / 2 : 8 * vq + vc / 4;
-      const int u0 = F8 ? wave * DT : 2 * wave * DT + (vc % 4) / 2;
-      const int va = vkey * T::LROW + ((u0 ^ swz_key<F8>(vkey)) * 16) + (vl & 1) * 8;
+      if constexpr (!EARLY) first_reads();
       if (wave == 0) *(lds_i32*)(lds + FLAGS + 4 * (buf ^ 1)) = 0;  // all have read it before this tile's barriers
 #pragma unroll
       for (int r = 0; r < MT; ++r) l[r] += sum[r];
-      // V fragments are read ahead of their MFMAs (the schedule is pinned: left to
-      // itself the compiler reads each where it is used, and every d tile waits out
-      // the LDS latency); the other half of the next tile's loads goes between.
-      {
-        constexpr int VN = 2 * DT, VAHEAD = 2, VRING = VAHEAD + 1;
-        v4s vlo[VRING], vhi[VRING];
-        v2i v8[VRING];
-        auto v_read = [&](int n) {
-          const int s2 = n / DT, t = n % DT;
-          if constexpr (F8) {
-            v8[n % VRING] = read_tr8(kb + (va ^ (t << 4)) + 32 * s2 * T::LROW);
-          } else {
-            vlo[n % VRING] = read_tr16(kb + (va ^ (t << 5)) + 32 * s2 * T::LROW);
-            vhi[n % VRING] = read_tr16(kb + (va ^ ((t << 5) | 16)) + (32 * s2 + 4) * T::LROW);  // keys + 4: swizzle bit 0
-          }
-        };
-        v8bf pf[MT];
+      if (tile + 2 < sg.t_end) st.fetch(p, tile + 2);
 #pragma unroll
-        for (int r = 0; r < MT; ++r) pf[r] = lds_v8bf(lds + PBUF + (16 * r + vc) * PROW + (8 * vq) * 2);
+      for (int n = 0; n < VN; ++n) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (n + VAHEAD < VN) v_read(n + VAHEAD);
+        if (EARLY && n == DT / 2) p_read(1);
+        __builtin_amdgcn_sched_barrier(0);
+        const v8bf vf = F8 ? widen_e4m3(v8[n % VRING]) : join_tr16(vlo[n % VRING], vhi[n % VRING]);
 #pragma unroll
-        for (int n = 0; n < VAHEAD; ++n) v_read(n);
-#pragma unroll
-        for (int n = 0; n < VN; ++n) {
-          __builtin_amdgcn_sched_barrier(0);
-          if (n + VAHEAD < VN) v_read(n + VAHEAD);
-          __builtin_amdgcn_sched_barrier(0);
-          const v8bf vf = F8 ? widen_e4m3(v8[n % VRING]) : join_tr16(vlo[n % VRING], vhi[n % VRING]);
-#pragma unroll
-          for (int r = 0; r < MT; ++r) {
-            o[r][n % DT] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[r], o[r][n % DT], 0, 0, 0);
-            if (n == DT - 1) pf[r] = lds_v8bf(lds + PBUF + (16 * r + vc) * PROW + (32 + 8 * vq) * 2);
-          }
+        for (int r = 0; r < MT; ++r) {
+          o[r][n % DT] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n / DT][r], o[r][n % DT], 0, 0, 0);
+          if (!EARLY && n == DT - 1) p_read(1, r, r + 1);
         }
       }
       if (more) {
-        st.finish(next, lds + SCL + (buf ^ 1) * 256);
-        if (tile + 2 < sg.t_end) st.fetch(p, tile + 2);
+        if (!whole) st.finish(next, lds + SCL + (buf ^ 1) * 256);
+        start(tile + 2);
       }
     }
 
@@ -731,7 +827,7 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
       if (poisoned) sum = __uint_as_float(0x7fc00000u);
       // a row that sees no key has a sum of 0: its output is 0 and its lse -inf
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      if (!whole) {
+      if (opaque_uniform(sg.t_begin) != 0 || sg.t_end != sg.tiles) {
         if (wave == 0 && el < 16)
           e.part_lse[slot * GROUP + member * ROWS + 16 * r + el] = sum == 0.0f ? -INFINITY : __builtin_fmaf(m[r], c2, log2f(sum));
         float4* po = (float4*)e.part_o + ((slot * (MT * PAIR) + member * MT + r) * (R / 16) + wave * DT) * 64 + el;
@@ -1021,6 +1117,15 @@ extern "C" int fcmoe_absorbed_attention(const fcmoe_absorbed_args* a, hipStream_
   p.part_lse = (float*)((char*)a->workspace + pl.joint_bytes);
   p.part_o = (float*)((char*)a->workspace + pl.joint_bytes + pl.lse_bytes);
   p.shares = (int)pl.shares;
+  // a page's rows, and the pages' distances, in 32 bits
+  const auto small = [&](int64_t page_stride, int64_t row_stride, int64_t bytes) {
+    return page_stride >= 0 && page_stride * bytes < ((int64_t)1 << 32) && row_stride < (1 << 24) &&
+           (row_stride * p.c.page_size + 1024) * bytes < ((int64_t)1 << 31);
+  };
+  const int64_t elem = p.c.e4m3 ? 1 : 2;
+  p.whole = p.c.page_size % 16 == 0 && small(p.c.latent_page_stride, p.c.latent_row_stride, elem) &&
+            (!p.c.rope_dim || small(p.c.rope_page_stride, p.c.rope_row_stride, elem)) &&
+            (!p.c.e4m3 || small(p.c.scale_page_stride, 1, 4));
   p.page_shift = -1;
   for (int i = 0; i <= 20; ++i)
     if (p.c.page_size == (int64_t)1 << i) p.page_shift = i;

@@ -77,13 +77,18 @@ __device__ __forceinline__ v8bf join_tr16(v4s lo, v4s hi) {
 
 // 16 bytes a lane from memory straight to LDS: lane l's land at dst + 16 l
 // (dst the same in all lanes). Counts in vmcnt. The second form reads a buffer
-// at a byte offset, zeros past its end.
+// at a byte offset, zeros past its end (which a part
+// that is the same for all lanes does not count against).
 __device__ __forceinline__ void load_lds16(const void* src, lds_u8* dst) {
   __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)src,
                                    (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
 }
-__device__ __forceinline__ void load_lds16(const __amdgpu_buffer_rsrc_t src, lds_u8* dst, uint32_t offset) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)dst, 16, offset, 0, 0, 0);
+__device__ __forceinline__ void load_lds16(const __amdgpu_buffer_rsrc_t src, lds_u8* dst, uint32_t offset,
+                                           uint32_t uniform_offset = 0) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)dst, 16, offset, uniform_offset, 0, 0);
+}
+__device__ __forceinline__ void load_lds4(const __amdgpu_buffer_rsrc_t src, lds_u8* dst, uint32_t offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)dst, 4, offset, 0, 0, 0);
 }
 
 template <int N>

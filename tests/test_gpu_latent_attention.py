@@ -337,6 +337,40 @@ def test_absorbed_long(gpu, lens, H, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("H,page", [(4, 32), (33, 24), (64, 64), (128, 16)])
+def test_absorbed_many_sequences(gpu, H, page, dtype):
+    """More sequences than a wave has lanes, and fewer row groups than shares, more, and about as many."""
+    for count in (70, 150, 290):
+        lens = [(37 * b) % 450 if b % 5 else 0 for b in range(count)]
+        lens[3], lens[count - 1] = 6000, 1
+        pg = _Paged(count, lens, 256, 64, dtype, page=page)
+        ql, qr = _queries(count, count, H, 256, 64)
+        out, lse = _check_absorbed(pg, lens, ql, qr, None, 0.07)
+        again = _la().absorbed_attention(ql, qr, pg.cache, pg.table, pg.lens, scale=0.07, return_lse=True)
+        assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_absorbed_shared_page_strides(gpu, dtype):
+    """A page that several table entries name, pages that lie on one another, and one row for all places of a page."""
+    la = _la()
+    lens = [300, 64, 129]
+    ql, qr = _queries(6, 3, 16, 512, 64)
+    pg = _Paged(22, [64], 512, 64, dtype, page=64)
+    table = pg.table.expand(3, -1)[:, :1].expand(3, 5)
+    got = la.absorbed_attention(ql, qr, pg.cache, table.contiguous(), _i32(lens), scale=0.07)
+    c = la.LatentCache(*(None if t is None else t[int(pg.table[0, 0])][None].expand(5, *t.shape[1:])
+                         for t in (pg.cache.latent, pg.cache.rope, pg.cache.scale)))
+    order = torch.arange(5, device="cuda", dtype=torch.int32)[None].expand(3, 5).contiguous()
+    assert torch.equal(la.absorbed_attention(ql, qr, c, order, _i32(lens), scale=0.07), got)
+    one = la.LatentCache(*(None if t is None else t[:, :1].expand(*t.shape) for t in (pg.cache.latent, pg.cache.rope)),
+                         None if pg.cache.scale is None else pg.cache.scale[:, :1].expand(*pg.cache.scale.shape).contiguous())
+    full = la.LatentCache(*(None if t is None else t.contiguous() for t in (one.latent, one.rope, one.scale)))
+    assert torch.equal(la.absorbed_attention(ql, qr, one, table.contiguous(), _i32(lens), scale=0.07),
+                       la.absorbed_attention(ql, qr, full, table.contiguous(), _i32(lens), scale=0.07))
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
 @pytest.mark.parametrize("H", [8, 32, 64, 128])
 def test_absorbed_growing_scores(gpu, H, dtype):
     """Each tile's scores far above the last one's, then far below: the running maximum moves tile by tile."""
