@@ -146,11 +146,25 @@ extern "C" int fcmoe_head_projection(const fcmoe_head_projection_args* a, hipStr
   p.n_tiles = (int)ceil_div(a->n, 16), p.k_chunks = (int)ceil_div(a->k, 32);
   if (ceil_div(a->tokens, 16) * a->heads * p.n_tiles > INT32_MAX)
     return fail(FCMOE_EINVAL, "head_projection: too many tokens");
+  // The largest tile of tokens x channels that still gives every SIMD a wave: a
+  // smaller one reads x and the weights more often, a larger one leaves the
+  // chip's other waves out. 128 heads, us: 512 -> 128 at 128 tokens 19, 16, 12,
+  // 15 (64 x 128, 64 x 64, 32 x 64, 32 x 32), at 300 23, 25, 26; 128 -> 512 at
+  // 48 tokens 9.3, 7.0 and, 48 x 64, 6.7, at 300 28, 25 (64 x 128 reads x fewer
+  // times, which is little where K < N: only past 4096 waves there); 16 heads,
+  // 512 -> 128 at 200 tokens 15, 12, 8, 7 and, 16 x 32, 5.
+  const auto waves = [&](int64_t mt, int64_t nt) { return ceil_div(a->tokens, 16 * mt) * a->heads * ceil_div(p.n_tiles, nt); };
   if (a->tokens <= 16)
     head_project_launch<1, 2>(p, stream);
-  else if (a->tokens <= 64)
-    head_project_launch<4, 2>(p, stream);
-  else
+  else if (waves(4, 8) >= (a->k < a->n ? 4096 : 512))
     head_project_launch<4, 8>(p, stream);
+  else if (waves(4, 4) >= 1024)
+    a->tokens <= 48 && a->tokens > 32 ? head_project_launch<3, 4>(p, stream) : head_project_launch<4, 4>(p, stream);
+  else if (waves(2, 4) >= 1024)
+    head_project_launch<2, 4>(p, stream);
+  else if (waves(2, 2) >= 1024)
+    head_project_launch<2, 2>(p, stream);
+  else
+    head_project_launch<1, 2>(p, stream);
   return check_launch("head_projection");
 }
