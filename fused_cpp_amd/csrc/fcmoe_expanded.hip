@@ -718,6 +718,9 @@ __global__ __launch_bounds__(kExpWaves * kWave, 1) void expanded_wide_kernel(con
 }
 
 // Joins the splits of a row block: out = sum_s 2^(lse_s - max) O_s / sum_s 2^(lse_s - max).
+// A workgroup takes 32 of the values (blockIdx.y): a CU takes some 10 bytes a clock
+// from beyond its L2, so the partials are read by many (two chunks of 65 tokens
+// behind 20000, 32 heads: 20 us a launch by one each, 11 so).
 template <int V>
 __global__ __launch_bounds__(kExpWaves * kWave) void expanded_combine_kernel(const Expanded p) {
   const int lane = (int)threadIdx.x % kWave, strips = p.rows / 32;
@@ -738,9 +741,11 @@ __global__ __launch_bounds__(kExpWaves * kWave) void expanded_combine_kernel(con
   float top = -INFINITY;
   for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_lse[(at + s * step) * 32 + lane % 32]);
   float total = 0.0f;
-  float4 acc[V / 8];
+  const int k0 = 4 * (int)blockIdx.y;
+  float4 acc[4];
 #pragma unroll
-  for (int k = 0; k < V / 8; ++k) acc[k] = make_float4(0, 0, 0, 0);
+  for (int k = 0; k < 4; ++k) acc[k] = make_float4(0, 0, 0, 0);
+#pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
     const float ls = p.part_lse[(at + s * step) * 32 + lane % 32];
     if (ls == -INFINITY) continue;  // no key of this split: nothing was stored that may be read
@@ -748,8 +753,8 @@ __global__ __launch_bounds__(kExpWaves * kWave) void expanded_combine_kernel(con
     total += w;
     const float4* po = (const float4*)p.part_o + (at + s * step) * (V / 8) * 64 + lane;
 #pragma unroll
-    for (int k = 0; k < V / 8; ++k) {
-      const float4 v = po[k * 64];
+    for (int k = 0; k < 4; ++k) {
+      const float4 v = po[(k0 + k) * 64];
       acc[k].x = __builtin_fmaf(w, v.x, acc[k].x);
       acc[k].y = __builtin_fmaf(w, v.y, acc[k].y);
       acc[k].z = __builtin_fmaf(w, v.z, acc[k].z);
@@ -758,11 +763,11 @@ __global__ __launch_bounds__(kExpWaves * kWave) void expanded_combine_kernel(con
   }
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   const int64_t token = seq.q0 + i;
-  if (p.lse && lane < 32) p.lse[token * p.heads + head] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
+  if (p.lse && blockIdx.y == 0 && lane < 32) p.lse[token * p.heads + head] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
   uint16_t* orow = p.out + token * p.ot + head * p.oh + 4 * (lane / 32);
 #pragma unroll
-  for (int k = 0; k < V / 8; ++k)
-    *(uint2*)(orow + 8 * k) = make_uint2(pack_bf16(acc[k].x * inv, acc[k].y * inv), pack_bf16(acc[k].z * inv, acc[k].w * inv));
+  for (int k = 0; k < 4; ++k)
+    *(uint2*)(orow + 8 * (k0 + k)) = make_uint2(pack_bf16(acc[k].x * inv, acc[k].y * inv), pack_bf16(acc[k].z * inv, acc[k].w * inv));
 }
 
 // Rows of a row block. 256 make two products of each K and V fragment read from
@@ -804,7 +809,7 @@ void expanded_launch(const Expanded& p, hipStream_t stream) {
   else
     hipLaunchKernelGGL((expanded_narrow_kernel<N, P, V>), grid, block, 0, stream, p);
   if (p.splits > 1)
-    hipLaunchKernelGGL((expanded_combine_kernel<V>), dim3((unsigned)(p.blocks * p.heads * (p.rows / 32 / kExpWaves))), block, 0,
+    hipLaunchKernelGGL((expanded_combine_kernel<V>), dim3((unsigned)(p.blocks * p.heads * (p.rows / 32 / kExpWaves)), V / 32), block, 0,
                        stream, p);
 }
 
