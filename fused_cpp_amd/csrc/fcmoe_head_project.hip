@@ -72,7 +72,8 @@ __global__ __launch_bounds__(kProjWaves * kWave) void head_project_kernel(const 
   // K is a multiple of 8: a lane's 8 values lie inside K or past it as a whole;
   // past it the packed weights are zero and x is taken as zero.
   const int full = p.K / 32;
-#pragma unroll 4
+  constexpr int AHEAD = MT * NT == 1 ? 16 : MT * NT == 4 ? 8 : 4;  // chunks whose loads are in flight together
+#pragma unroll AHEAD
   for (int c = 0; c < full; ++c) {
     v8bf xf[MT], wf[NT];
 #pragma unroll
@@ -147,24 +148,24 @@ extern "C" int fcmoe_head_projection(const fcmoe_head_projection_args* a, hipStr
   if (ceil_div(a->tokens, 16) * a->heads * p.n_tiles > INT32_MAX)
     return fail(FCMOE_EINVAL, "head_projection: too many tokens");
   // The largest tile of tokens x channels that still gives every SIMD a wave: a
-  // smaller one reads x and the weights more often, a larger one leaves the
-  // chip's other waves out. 128 heads, us: 512 -> 128 at 128 tokens 19, 16, 12,
-  // 15 (64 x 128, 64 x 64, 32 x 64, 32 x 32), at 300 23, 25, 26; 128 -> 512 at
-  // 48 tokens 9.3, 7.0 and, 48 x 64, 6.7, at 300 28, 25 (64 x 128 reads x fewer
-  // times, which is little where K < N: only past 4096 waves there); 16 heads,
-  // 512 -> 128 at 200 tokens 15, 12, 8, 7 and, 16 x 32, 5.
+  // smaller one reads x and the weights more often, a larger one leaves too few
+  // loads in flight. 128 heads with weights from memory, us: 128 -> 512 at 1
+  // token 7.0, 5.9, 5.6 (64 x 64, 32 x 32, 16 x 16), at 32 8.9, 7.1, 9.2, at 48
+  // 9.7, 11.2 and, 48 x 64, 9.5, at 300 29, 37; 64 x 128 reads x fewer times, little
+  // where K < N: 32, there only past 4096 waves. 512 -> 128 at 48 tokens 18, 12.3,
+  // 12.0, at 100 19, 15, 19 and, 32 x 64, 14, at 300 30, 40 and, 64 x 128, 28.
   const auto waves = [&](int64_t mt, int64_t nt) { return ceil_div(a->tokens, 16 * mt) * a->heads * ceil_div(p.n_tiles, nt); };
   if (a->tokens <= 16)
-    head_project_launch<1, 2>(p, stream);
-  else if (waves(4, 8) >= (a->k < a->n ? 4096 : 512))
+    head_project_launch<1, 1>(p, stream);
+  else if (a->tokens > 32 && waves(4, 8) >= (a->k < a->n ? 4096 : 640))
     head_project_launch<4, 8>(p, stream);
-  else if (waves(4, 4) >= 1024)
-    a->tokens <= 48 && a->tokens > 32 ? head_project_launch<3, 4>(p, stream) : head_project_launch<4, 4>(p, stream);
-  else if (waves(2, 4) >= 1024)
+  else if (a->tokens > 32 && waves(4, 4) >= 1024)
+    a->tokens <= 48 ? head_project_launch<3, 4>(p, stream) : head_project_launch<4, 4>(p, stream);
+  else if (a->tokens > 32 && waves(2, 4) >= 1024)
     head_project_launch<2, 4>(p, stream);
   else if (waves(2, 2) >= 1024)
     head_project_launch<2, 2>(p, stream);
   else
-    head_project_launch<1, 2>(p, stream);
+    head_project_launch<1, 1>(p, stream);
   return check_launch("head_projection");
 }
