@@ -659,6 +659,7 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
             }
           });
         }
+        if constexpr (MT > 1) qk_done<MT>(s);
       };
       if (whole)
         scores(std::integral_constant<int, 2>{});
@@ -666,7 +667,6 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
         scores(std::integral_constant<int, 1>{});
       else
         scores(std::integral_constant<int, 0>{});
-      if constexpr (MT > 1) qk_done<MT>(s);
       if (whole)
         st.scales_whole(lds + SCL + (buf ^ 1) * 256);
       else if (more)

@@ -151,7 +151,7 @@ extern "C" int fcmoe_head_projection(const fcmoe_head_projection_args* a, hipStr
   // smaller one reads x and the weights more often, a larger one leaves too few
   // loads in flight. 128 heads with weights from memory, us: 128 -> 512 at 1
   // token 7.0, 5.9, 5.6 (64 x 64, 32 x 32, 16 x 16), at 32 8.9, 7.1, 9.2, at 48
-  // 9.7, 11.2 and, 48 x 64, 9.5, at 300 29, 37; 64 x 128 reads x fewer times, little
+  // 9.7, 11.2 and, 48 x 32, 9.6 (a call alone 8.3, 48 x 64 8.9), at 300 29, 37; 64 x 128 reads x fewer times, little
   // where K < N: 32, there only past 4096 waves. 512 -> 128 at 48 tokens 18, 12.3,
   // 12.0, at 100 19, 15, 19 and, 32 x 64, 14, at 300 30, 40 and, 64 x 128, 28.
   const auto waves = [&](int64_t mt, int64_t nt) { return ceil_div(a->tokens, 16 * mt) * a->heads * ceil_div(p.n_tiles, nt); };
@@ -160,7 +160,7 @@ extern "C" int fcmoe_head_projection(const fcmoe_head_projection_args* a, hipStr
   else if (a->tokens > 32 && waves(4, 8) >= (a->k < a->n ? 4096 : 640))
     head_project_launch<4, 8>(p, stream);
   else if (a->tokens > 32 && waves(4, 4) >= 1024)
-    a->tokens <= 48 ? head_project_launch<3, 4>(p, stream) : head_project_launch<4, 4>(p, stream);
+    a->tokens <= 48 ? head_project_launch<3, 2>(p, stream) : head_project_launch<4, 4>(p, stream);
   else if (a->tokens > 32 && waves(2, 4) >= 1024)
     head_project_launch<2, 4>(p, stream);
   else if (waves(2, 2) >= 1024)

@@ -157,7 +157,8 @@ def expanded_attention(q: torch.Tensor, kv: torch.Tensor, k_rope: Optional[torch
 
     Sequences are packed: ``query_starts [B + 1]`` and ``kv_starts [B + 1]`` int32 (default: the same) bound their
     query tokens and keys. With ``causal`` query i of n sees the first ``keys - n + i + 1`` keys. ``nope`` and ``v``
-    are both 128 or both 64, ``rope_dim`` 64 or none. Empty rows, ``return_lse`` and ``out`` as in
+    are both 128 or both 64, ``rope_dim`` 64 or none. Keys and values that a sequence's queries do not all see have to
+    be finite; what no sequence holds may be anything. Empty rows, ``return_lse`` and ``out`` as in
     :func:`absorbed_attention`.
     """
     o, lse = _native.require_native().latent_expanded_attention(q, kv, k_rope, query_starts, kv_starts, scale, causal,
