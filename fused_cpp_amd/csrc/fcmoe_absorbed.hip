@@ -74,7 +74,7 @@ __device__ __forceinline__ SeqSpan absorbed_span(const Absorbed& p, int b) {
   SeqSpan s;
   if (p.q_starts) {
     s.q0 = clamp64(p.q_starts[b], 0, p.tokens);
-    s.n = (int)(clamp64(p.q_starts[b + 1], s.q0, p.tokens) - s.q0);
+    s.n = (int)(clamp64(p.q_starts[b + 1], 0, p.tokens) - s.q0);
   } else {
     s.q0 = b;
     s.n = b < p.tokens ? 1 : 0;
@@ -416,13 +416,16 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
   __shared__ __align__(1024) uint8_t smem[QFITS || MT == 1 ? FLAGS + 16 : QOFF + ROWS * 2 * (R + P)];
   lds_u8* lds = (lds_u8*)smem;
   const int wave = wave_index();
-  if (p.zero_tail)
-    zero_uncovered(p.q_starts, p.batch, p.tokens, p.heads, R, p.out, p.ot, p.oh, p.lse, blockIdx.x, gridDim.x);
-
-  const int64_t units = count_items(
-      p.batch, [&](int b) { return absorbed_span(p, b); },
-      [&](const SeqSpan& q) { return (int64_t)row_groups(p, q, GROUP) * group_units(q); });
-  const int64_t shares = units < p.shares ? units : p.shares;
+  int64_t units, shares;
+  {
+    const Absorbed a = args_now();
+    if (a.zero_tail)
+      zero_uncovered(a.q_starts, a.batch, a.tokens, a.heads, R, a.out, a.ot, a.oh, a.lse, blockIdx.x, gridDim.x);
+    units = count_items(
+        a.batch, [&](int b) { return absorbed_span(a, b); },
+        [&](const SeqSpan& q) { return (int64_t)row_groups(a, q, GROUP) * group_units(q); });
+    shares = units < a.shares ? units : a.shares;
+  }
   // workgroups go to the 8 XCDs by blockIdx % 8: a pair's two are 8 apart
   const int member = PAIR == 2 ? (int)(blockIdx.x / 8 % 2) : 0;
   const int64_t g = PAIR == 2 ? blockIdx.x / 16 * 8 + blockIdx.x % 8 : blockIdx.x;

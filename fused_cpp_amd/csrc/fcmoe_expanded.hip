@@ -65,7 +65,7 @@ struct Expanded {
 __device__ __forceinline__ SeqSpan expanded_span(const Expanded& p, int b) {
   SeqSpan s;
   s.q0 = clamp64(p.q_starts[b], 0, p.tokens);
-  s.n = (int)(clamp64(p.q_starts[b + 1], s.q0, p.tokens) - s.q0);
+  s.n = (int)(clamp64(p.q_starts[b + 1], 0, p.tokens) - s.q0);
   s.k0 = clamp64(p.kv_starts[b], 0, p.keys);
   s.len = (int)(clamp64(p.kv_starts[b + 1], s.k0, p.keys) - s.k0);
   return s;

@@ -155,10 +155,10 @@ __device__ __forceinline__ uint64_t lane_value(uint64_t v, int l) {
 }
 
 // Lengths that the device reads are bounded here, so that no value of them
-// leads a kernel outside the tensors the host has checked.
+// leads a kernel outside the tensors and workspaces the host has checked.
 struct SeqSpan {
   int64_t q0;  // first query token
-  int n;       // query tokens
+  int n;       // query tokens; below 0 where the next start lies below this one, until follow()
   int64_t k0;  // first key (expanded form)
   int len;     // keys
 };
@@ -186,20 +186,49 @@ __device__ __forceinline__ int64_t wave_scan(int64_t v) {
   return v;
 }
 
+// Inclusive maximum over the wave's lanes of values that are not negative.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int max_dpp(int v) {
+  return max(v, __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, true));
+}
+__device__ __forceinline__ int wave_scan_max(int v) {
+  v = max_dpp<0x111, 0xf>(v);
+  v = max_dpp<0x112, 0xf>(v);
+  v = max_dpp<0x114, 0xf>(v);
+  v = max_dpp<0x118, 0xf>(v);
+  v = max_dpp<0x142, 0xa>(v);
+  v = max_dpp<0x143, 0xc>(v);
+  return v;
+}
+
+// Query spans of 64 neighbouring sequences, one a lane, made to follow one
+// another: a start below an earlier one counts as that one. So no token belongs
+// to two sequences, and a batch has no more rows than tokens whatever the
+// starts are, which is what row groups, row blocks and workspaces are counted
+// by. `high` is the largest start before these sequences; returns the one
+// behind them. Starts in order cost a compare a lane.
+__device__ __forceinline__ int follow(SeqSpan& s, int high) {
+  if (__any(s.n < 0 || s.q0 < high)) {
+    const int end = (int)s.q0 + s.n, first = max(high, wave_scan_max((int)s.q0));
+    s.q0 = first;
+    s.n = max(end - first, 0);
+  }
+  return __builtin_amdgcn_readlane((int)s.q0 + s.n, kWave - 1);
+}
+
 // Finds the sequence that item `item` (0 <= item) falls into, where a sequence
 // with span s holds count(s) items: its index and span and the items before it;
 // -1 past the last. The whole wave takes part and gets the same answer.
 template <typename S, typename F>
 __device__ __forceinline__ int find_sequence(int batch, int64_t item, S span, F count, SeqSpan* found, int64_t* before) {
   int64_t base = 0;
+  int high = 0;
   for (int b0 = 0; b0 < batch; b0 += kWave) {
     const int b = b0 + lane_now();
-    SeqSpan s{};
-    int64_t mine = 0;
-    if (b < batch) {
-      s = span(b);
-      mine = count(s);
-    }
+    SeqSpan s{high, 0, 0, 0};
+    if (b < batch) s = span(b);
+    high = follow(s, high);
+    const int64_t mine = b < batch ? count(s) : 0;
     const int64_t upto = base + wave_scan(mine);
     const uint64_t hit = __ballot(upto > item);
     if (hit) {
@@ -220,19 +249,30 @@ __device__ __forceinline__ int find_sequence(int batch, int64_t item, S span, F 
 template <typename S, typename F>
 __device__ __forceinline__ int64_t count_items(int batch, S span, F count) {
   int64_t sum = 0;
-  for (int b = lane_now(); b < batch; b += kWave) sum += count(span(b));
+  int high = 0;
+  for (int b0 = 0; b0 < batch; b0 += kWave) {
+    const int b = b0 + lane_now();
+    SeqSpan s{high, 0, 0, 0};
+    if (b < batch) s = span(b);
+    high = follow(s, high);
+    sum += b < batch ? count(s) : 0;
+  }
   return (int64_t)lane_value((uint64_t)wave_scan(sum), kWave - 1);
 }
 
-// Tokens that no sequence holds (before the first start, behind the last)
+// Tokens that no sequence holds (before the first start, behind the largest)
 // become zero, their lse -inf: the workgroups of an attention launch share
 // them out, `wg` of `wgs`. For outputs that the call allocates; a caller's own
 // output keeps those rows.
 __device__ __forceinline__ void zero_uncovered(const int32_t* starts, int batch, int64_t tokens, int heads, int dim,
                                                uint16_t* out, int64_t ot, int64_t oh, float* lse, int64_t wg,
                                                int64_t wgs) {
-  const int64_t first = clamp64(starts[0], 0, tokens), end = clamp64(starts[batch], 0, tokens);
+  const int64_t first = clamp64(starts[0], 0, tokens);
+  int64_t end = clamp64(starts[batch], 0, tokens);
   if (first == 0 && end == tokens) return;
+  int top = (int)end;
+  for (int b = lane_now(); b < batch; b += kWave) top = max(top, (int)clamp64(starts[b], 0, tokens));
+  end = __builtin_amdgcn_readlane(wave_scan_max(top), kWave - 1);
   for (int64_t t = wg; t < tokens; t += wgs) {
     if (t >= first && t < end) continue;
     for (int k = (int)threadIdx.x; k < heads * (dim / 4); k += (int)blockDim.x) {

@@ -135,10 +135,11 @@ def absorbed_attention(q_latent: torch.Tensor, q_rope: Optional[torch.Tensor], c
 
     ``q_latent [T, H, latent_dim]`` and ``q_rope [T, H, rope_dim]`` (``None`` without a separate key part).
     ``page_table [B, width]`` int32, ``kv_lens [B]`` int32: cached tokens of each sequence, this call's included.
-    ``query_starts [B + 1]`` int32: sequence b's query tokens; without it each sequence has one. Query i of n sees the
-    first ``kv_lens[b] - n + i + 1`` tokens; one that sees none is 0. Lengths past the table's reach are cut to it, a
-    page id outside the cache makes its sequence NaN. Cached tokens that a sequence's queries do not all see have to
-    be finite; rows past a length may hold anything.
+    ``query_starts [B + 1]`` int32: sequence b's query tokens; without it each sequence has one. Starts are cut to the
+    tokens there are, and one below an earlier one counts as that one: a batch may be padded with any of either. Query
+    i of n sees the first ``kv_lens[b] - n + i + 1`` tokens; one that sees none is 0. Lengths past the table's reach are
+    cut to it, a page id outside the cache makes its sequence NaN. Cached tokens that a sequence's queries do not all
+    see have to be finite; rows past a length may hold anything.
 
     ``return_lse`` adds ``[T, H]`` fp32: the log of the softmax's sum (-inf where there is none), which joins results
     over parts of a context. Tokens that no sequence holds are 0, or left as they were in a given ``out``.
@@ -156,10 +157,10 @@ def expanded_attention(q: torch.Tensor, kv: torch.Tensor, k_rope: Optional[torch
     the heads share (``None`` without one): ``[T, H, v]`` from ``q [T, H, nope + rope_dim]``.
 
     Sequences are packed: ``query_starts [B + 1]`` and ``kv_starts [B + 1]`` int32 (default: the same) bound their
-    query tokens and keys. With ``causal`` query i of n sees the first ``keys - n + i + 1`` keys. ``nope`` and ``v``
-    are both 128 or both 64, ``rope_dim`` 64 or none. Keys and values that a sequence's queries do not all see have to
-    be finite; what no sequence holds may be anything. Empty rows, ``return_lse`` and ``out`` as in
-    :func:`absorbed_attention`.
+    query tokens and keys, query starts as in :func:`absorbed_attention`. With ``causal`` query i of n sees the
+    first ``keys - n + i + 1`` keys. ``nope`` and ``v`` are both 128 or both 64, ``rope_dim`` 64 or none. Keys and values
+    that a sequence's queries do not all see have to be finite; what no sequence holds may be anything. Empty rows,
+    ``return_lse`` and ``out`` as in :func:`absorbed_attention`.
     """
     o, lse = _native.require_native().latent_expanded_attention(q, kv, k_rope, query_starts, kv_starts, scale, causal,
                                                                 out, return_lse)

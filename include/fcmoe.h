@@ -293,8 +293,9 @@ int fcmoe_head_projection(const fcmoe_head_projection_args* args, hipStream_t st
  *   s_j = scale * (q_latent . c_j + q_rope . r_j),  out = sum_j softmax(s)_j c_j,
  * where page page_table[b, j / page_size] holds token j. out [tokens, heads,
  * latent_dim]; lse [tokens, heads] fp32 (optional): log sum_j exp(s_j). A row
- * that sees no token is 0 with lse -inf. Lengths past the page table's reach
- * are cut to it. A page id outside the cache that a length reaches makes the
+ * that sees no token is 0 with lse -inf. Query starts are cut to the tokens, and
+ * one below an earlier one counts as that one, so that no token is held twice.
+ * Lengths past the page table's reach are cut to it. A page id outside the cache that a length reaches makes the
  * sequence's rows NaN. Rows past a length may hold anything; a cached token
  * that some query of a sequence sees has to be finite for the others too.
  * zero_uncovered: tokens that no sequence holds become 0 (else they are left).
