@@ -5,15 +5,16 @@
 // the kernels' 16-byte loads need them, allocates outputs and workspaces from
 // the torch caching allocator on the current stream of the tensors' device and
 // calls the C ABI of libfcmoe.so.
-#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "../../include/fcmoe.h"
 
@@ -77,6 +78,100 @@ int64_t stride_at(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.str
 
 const uint16_t* bf16(const at::Tensor& t) { return t.defined() ? (const uint16_t*)t.data_ptr() : nullptr; }
 
+// Whether strided tensors share memory, exactly: is there a t with
+// distance + sum_i step_i t_i = 0 and low_i <= t_i <= high_i? Steps are taken
+// from the largest down; what the smaller ones can still add bounds each t_i to
+// a few values where dimensions lie inside one another, as views' do. Layouts
+// so entangled that the search is long count as sharing.
+class Reach {
+ public:
+  void add(int64_t step, int64_t low, int64_t high) {
+    if (low == high && low == 0) return;
+    for (Term& t : terms_)
+      if (t.step == step) {
+        t.low += low, t.high += high;
+        return;
+      }
+    terms_.push_back({step, low, high});
+  }
+  bool zero(int64_t distance) {
+    std::sort(terms_.begin(), terms_.end(), [](const Term& a, const Term& b) { return a.step > b.step; });
+    const size_t n = terms_.size();
+    rest_low_.assign(n + 1, 0), rest_high_.assign(n + 1, 0);
+    for (size_t i = n; i-- > 0;) {
+      rest_low_[i] = rest_low_[i + 1] + terms_[i].step * terms_[i].low;
+      rest_high_[i] = rest_high_[i + 1] + terms_[i].step * terms_[i].high;
+    }
+    left_ = 1 << 18;
+    return from(0, distance);
+  }
+
+ private:
+  struct Term {
+    int64_t step, low, high;
+  };
+  static int64_t floor_div(int64_t a, int64_t b) { return a >= 0 ? a / b : -((-a + b - 1) / b); }
+  bool from(size_t i, int64_t d) {
+    if (i == terms_.size()) return d == 0;
+    const Term& t = terms_[i];
+    if (t.step == 0) return from(i + 1, d);
+    const int64_t first = std::max(t.low, -floor_div(d + rest_high_[i + 1], t.step));
+    const int64_t last = std::min(t.high, floor_div(-d - rest_low_[i + 1], t.step));
+    for (int64_t v = first; v <= last; ++v) {
+      if (--left_ < 0) return true;
+      if (from(i + 1, d + v * t.step)) return true;
+    }
+    return false;
+  }
+  std::vector<Term> terms_;
+  std::vector<int64_t> rest_low_, rest_high_;
+  int64_t left_ = 0;
+};
+
+int64_t address(const at::Tensor& t) { return (int64_t)reinterpret_cast<uintptr_t>(t.data_ptr()); }
+int64_t byte_stride(const at::Tensor& t, int64_t d) { return t.stride(d) * (int64_t)t.element_size(); }
+// Bytes from the first to behind the last.
+int64_t extent(const at::Tensor& t) {
+  int64_t e = (int64_t)t.element_size();
+  for (int64_t d = 0; d < t.dim(); ++d) e += (t.size(d) - 1) * byte_stride(t, d);
+  return e;
+}
+
+bool share_memory(const at::Tensor& a, const at::Tensor& b) {
+  if (!a.defined() || !b.defined() || a.device() != b.device() || a.numel() == 0 || b.numel() == 0) return false;
+  const int64_t at_a = address(a), at_b = address(b);
+  if (at_a + extent(a) <= at_b || at_b + extent(b) <= at_a) return false;
+  Reach r;
+  for (int64_t d = 0; d < a.dim(); ++d) r.add(byte_stride(a, d), -(a.size(d) - 1), 0);
+  for (int64_t d = 0; d < b.dim(); ++d) r.add(byte_stride(b, d), 0, b.size(d) - 1);
+  r.add(1, -((int64_t)a.element_size() - 1), (int64_t)b.element_size() - 1);
+  return r.zero(at_b - at_a);
+}
+
+// Whether two places of a tensor are one: two index vectors that differ first
+// in dimension `d` (by 1 and more; the others by anything) and meet.
+bool shares_itself(const at::Tensor& t) {
+  if (t.numel() < 2) return false;
+  for (int64_t d = 0; d < t.dim(); ++d) {
+    if (t.size(d) < 2) continue;
+    if (t.stride(d) == 0) return true;
+    Reach r;
+    for (int64_t e = d + 1; e < t.dim(); ++e) r.add(byte_stride(t, e), -(t.size(e) - 1), t.size(e) - 1);
+    r.add(byte_stride(t, d), 0, t.size(d) - 2);
+    if (r.zero(byte_stride(t, d))) return true;
+  }
+  return false;
+}
+
+// What a call writes lies apart from what it reads, and no two of its places are one.
+void check_written(const at::Tensor& written, const char* name, std::initializer_list<const at::Tensor*> others,
+                   const char* what) {
+  if (!written.defined()) return;
+  TORCH_CHECK(!shares_itself(written), what, ": ", name, " must not overlap itself");
+  for (const at::Tensor* t : others)
+    TORCH_CHECK(!share_memory(written, *t), what, ": ", name, " must not overlap the call's other tensors");
+}
+
 // A caller's output, or a new one. `direct` is what the kernel writes: the
 // output itself where its rows can be stored in place, else a copy of it that
 // is copied back (so that rows the call leaves alone keep their values).
@@ -100,7 +195,6 @@ void check_output(const OptTensor& out, at::IntArrayRef sizes, const char* what)
   TORCH_CHECK_TYPE(out->scalar_type() == at::kBFloat16, what, ": out must be bfloat16, got ", out->scalar_type());
   TORCH_CHECK_VALUE(out->sizes() == sizes, what, ": out must be ", sizes, ", got ", out->sizes());
   TORCH_CHECK(!out->requires_grad(), what, ": out with requires_grad=True is not supported");
-  at::assert_no_internal_overlap(*out);
 }
 void finish(Out& o) {
   if (!o.direct.is_same(o.result)) o.result.copy_(o.direct);
@@ -142,12 +236,11 @@ at::Tensor head_norm_rope(at::Tensor x, at::Tensor positions, at::Tensor cos_sin
   check_output(out, x.sizes(), what);
   const at::Tensor w = opt(weight), given = opt(out);
   check_no_grad({&x, &cos_sin, &w}, what);
-  if (given.defined()) {
-    const bool same = given.data_ptr() == x.data_ptr() && given.strides() == x.strides();
-    TORCH_CHECK(same || at::get_overlap_status(given, x) == at::MemOverlapStatus::No ||
-                    at::get_overlap_status(given, x) == at::MemOverlapStatus::TooHard,
-                what, ": out must be x itself or not overlap it");
-  }
+  // in place: a row is read by the lanes that write it, before they do
+  const bool in_place = given.defined() && given.data_ptr() == x.data_ptr() && stride_at(given, 0) == stride_at(x, 0) &&
+                        stride_at(given, 1) == stride_at(x, 1) && stride_at(given, 2) == stride_at(x, 2);
+  const at::Tensor none;
+  check_written(given, "out (unless it is x itself)", {in_place ? &none : &x, &positions, &cos_sin, &w}, what);
   check_devices(x, {&positions, &cos_sin, &w, &given}, what);
   c10::DeviceGuard guard(x.device());
   Out o = output(out, x.sizes(), x, 1, what);
@@ -220,9 +313,6 @@ OptTensor latent_cache_append(at::Tensor kv, at::Tensor positions, at::Tensor sl
   const at::Tensor rope = opt(rope_), scale = opt(scale_), w = opt(weight);
   fcmoe_latent_append_args a{};
   a.cache = check_cache(latent, rope, scale, what);
-  at::assert_no_internal_overlap(latent);
-  if (rope.defined()) at::assert_no_internal_overlap(rope);
-  if (scale.defined()) at::assert_no_internal_overlap(scale);
   check_dtype(kv, at::kBFloat16, "kv");
   const int64_t W = a.cache.latent_dim + a.cache.rope_dim;
   TORCH_CHECK_VALUE(kv.dim() == 2 && kv.size(1) == W, "kv must be [tokens, ", W, "], got ", kv.sizes());
@@ -245,6 +335,9 @@ OptTensor latent_cache_append(at::Tensor kv, at::Tensor positions, at::Tensor sl
                       w.sizes());
   }
   check_no_grad({&kv, &cos_sin, &w, &latent, &rope, &scale}, what);
+  check_written(latent, "cache.latent", {&rope, &scale, &kv, &positions, &slots, &cos_sin, &w}, what);
+  check_written(rope, "cache.rope", {&scale, &kv, &positions, &slots, &cos_sin, &w}, what);
+  check_written(scale, "cache.scale", {&kv, &positions, &slots, &cos_sin, &w}, what);
   check_devices(kv, {&positions, &slots, &cos_sin, &latent, &rope, &scale, &w}, what);
   c10::DeviceGuard guard(kv.device());
   OptTensor rows;
@@ -294,7 +387,7 @@ at::Tensor head_projection(at::Tensor x, at::Tensor packed, int64_t heads, int64
   check_output(out, {T, heads, n}, what);
   const at::Tensor given = opt(out);
   check_no_grad({&x}, what);
-  if (given.defined()) at::assert_no_overlap(given, x);
+  check_written(given, "out", {&x, &packed}, what);
   check_devices(x, {&packed, &given}, what);
   c10::DeviceGuard guard(x.device());
   Out o = output(out, {T, heads, n}, x, 4, what);
@@ -360,11 +453,8 @@ std::tuple<at::Tensor, OptTensor> absorbed_attention(at::Tensor q_latent, OptTen
   check_output(out, {T, H, R}, what);
   const at::Tensor given = opt(out);
   check_no_grad({&q_latent, &q_rope, &latent, &rope, &cache_scale}, what);
+  check_written(given, "out", {&q_latent, &q_rope, &latent, &rope, &cache_scale, &page_table, &kv_lens, &starts}, what);
   check_devices(q_latent, {&q_rope, &latent, &rope, &cache_scale, &page_table, &kv_lens, &starts, &given}, what);
-  if (given.defined()) {
-    at::assert_no_overlap(given, q_latent);
-    if (q_rope.defined()) at::assert_no_overlap(given, q_rope);
-  }
   c10::DeviceGuard guard(q_latent.device());
   Out o = output(out, {T, H, R}, q_latent, 4, what);
   OptTensor lse;
@@ -433,12 +523,8 @@ std::tuple<at::Tensor, OptTensor> expanded_attention(at::Tensor q, at::Tensor kv
   check_output(out, {T, H, V}, what);
   const at::Tensor given = opt(out);
   check_no_grad({&q, &kv, &k_rope}, what);
+  check_written(given, "out", {&q, &kv, &k_rope, &query_starts, &kv_starts}, what);
   check_devices(q, {&kv, &k_rope, &query_starts, &kv_starts, &given}, what);
-  if (given.defined()) {
-    at::assert_no_overlap(given, q);
-    at::assert_no_overlap(given, kv);
-    if (k_rope.defined()) at::assert_no_overlap(given, k_rope);
-  }
   c10::DeviceGuard guard(q.device());
   Out o = output(out, {T, H, V}, q, 4, what);
   OptTensor lse;

@@ -24,7 +24,9 @@ Everything is bf16 in and out with fp32 arithmetic; the cache is bf16, or e4m3
 with one fp32 scale a token. Inference only: inputs that require a gradient are
 refused while gradients are recorded. Calls run on the current stream of their
 tensors' device, allocate through torch, read lengths, positions, slots and
-page ids on the device only, and can be captured into a HIP graph.
+page ids on the device only, and can be captured into a HIP graph. What a call
+writes may lie between the rows of what it reads, as views of one tensor do,
+but share no memory with it.
 """
 
 from __future__ import annotations
@@ -90,7 +92,7 @@ def head_norm_rope(x: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tens
     ``cos_sin.shape[1]`` values of a head turn by the angles of table row ``positions[t]``: ``cos_sin
     [positions, rope_dim]`` fp32 holds the cosines of the pairs, then their sines. Pairs are neighbours
     (``interleaved``) or half the rotated part apart; ``inverse`` turns back. A position outside the table makes the
-    rotated values NaN. ``out`` may be ``x``.
+    rotated values NaN. ``out`` may be ``x`` itself.
     """
     return _native.require_native().latent_head_norm_rope(x, positions, cos_sin, weight, eps, normalize, inverse,
                                                           interleaved, out)

@@ -208,7 +208,8 @@ int fcmoe_i8gemm_pair(const uint16_t* x, int64_t m, int64_t k, const void* w1_pa
  * The steps between the W8A8 projections of a DeepSeek latent-attention layer:
  * what the reference's adapter leaves to its caller's attention backend. No
  * counterpart in the fused-MoE reference path. All tensors are bf16 unless
- * stated; strides are in elements, the last dimension is contiguous. */
+ * stated; strides are in elements, the last dimension is contiguous. What a
+ * call writes shares no memory with what it reads. */
 
 /* Per-head RMS norm and position rotation of x [tokens, heads, dim], one pass:
  * y = x * rsqrt(mean(x^2) + eps) * weight (normalize != 0; weight optional),
@@ -216,7 +217,7 @@ int fcmoe_i8gemm_pair(const uint16_t* x, int64_t m, int64_t k, const void* w1_pa
  * table row positions[token]: cos_sin [table_rows, rope_dim] fp32, cosines of
  * the rope_dim / 2 pairs, then their sines. interleaved: pairs are
  * neighbours; else rope_dim / 2 apart. inverse: by the negative angles. A
- * position outside the table makes the rotated values NaN. out may be x. */
+ * position outside the table makes the rotated values NaN. out may be x itself. */
 typedef struct fcmoe_head_norm_rope_args {
   const uint16_t* x;
   int64_t tokens, heads, dim;
