@@ -6,6 +6,7 @@
 // the torch caching allocator on the current stream of the tensors' device and
 // calls the C ABI of libfcmoe.so.
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
@@ -42,12 +43,21 @@ void check_index(const at::Tensor& t, int64_t size, const char* name) {
   TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == size, name, " must be [", size, "], got ", t.sizes());
 }
 
-// Inference operators: a result that silently has no gradient is refused.
+// Inference operators: a result that silently has no gradient, or no tangent
+// of forward-mode differentiation, is refused.
+bool has_tangent(const at::Tensor& t) {
+  return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t.defined() && t._fw_grad(0).defined();
+}
 void check_no_grad(std::initializer_list<const at::Tensor*> ts, const char* what) {
-  if (!c10::GradMode::is_enabled()) return;
-  for (const at::Tensor* t : ts)
-    TORCH_CHECK(!t->defined() || !t->requires_grad(), what,
+  for (const at::Tensor* t : ts) {
+    TORCH_CHECK(!c10::GradMode::is_enabled() || !t->defined() || !t->requires_grad(), what,
                 ": inputs that require a gradient are not supported (use torch.no_grad())");
+    TORCH_CHECK(!has_tangent(*t), what, ": inputs with a forward-mode tangent are not supported");
+  }
+}
+// A tensor that a kernel wrote to: a graph that saved it before finds out.
+void was_written(const at::Tensor& t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 void check_devices(const at::Tensor& first, std::initializer_list<const at::Tensor*> ts, const char* what) {
@@ -194,10 +204,13 @@ void check_output(const OptTensor& out, at::IntArrayRef sizes, const char* what)
   if (!has(out)) return;
   TORCH_CHECK_TYPE(out->scalar_type() == at::kBFloat16, what, ": out must be bfloat16, got ", out->scalar_type());
   TORCH_CHECK_VALUE(out->sizes() == sizes, what, ": out must be ", sizes, ", got ", out->sizes());
-  TORCH_CHECK(!out->requires_grad(), what, ": out with requires_grad=True is not supported");
+  TORCH_CHECK(!out->requires_grad() && !has_tangent(*out), what, ": out with requires_grad=True is not supported, nor one with a tangent");
 }
 void finish(Out& o) {
-  if (!o.direct.is_same(o.result)) o.result.copy_(o.direct);
+  if (!o.direct.is_same(o.result))
+    o.result.copy_(o.direct);
+  else if (o.given)
+    was_written(o.result);
 }
 
 void check_table(const at::Tensor& cos_sin) {
@@ -354,8 +367,13 @@ OptTensor latent_cache_append(at::Tensor kv, at::Tensor positions, at::Tensor sl
   a.table_rows = table.size(0), a.rot_dim = table.size(1);
   a.weight = bf16(ws), a.eps = (float)eps, a.interleaved = interleaved;
   a.rows_out = return_rows ? (uint16_t*)rows->data_ptr() : nullptr;
-  pybind11::gil_scoped_release release;
-  check_rc(fcmoe_latent_cache_append(&a, stream_of(kv)), what);
+  {
+    pybind11::gil_scoped_release release;
+    check_rc(fcmoe_latent_cache_append(&a, stream_of(kv)), what);
+  }
+  was_written(latent);
+  was_written(rope);
+  was_written(scale);
   return rows;
 }
 
