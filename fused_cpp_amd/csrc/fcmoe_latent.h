@@ -128,11 +128,11 @@ __device__ __forceinline__ int opaque_uniform(int v) {
   asm volatile("" : "+s"(v));
   return v;
 }
-// The lane's number, formed anew: what depends on it is neither kept in a register nor hoisted past this point.
+// The lane's number, formed anew: what depends on it is neither kept in a register nor hoisted past this point. (The
+// instructions are the compiler's, which puts the waits around them that a product in flight asks for.)
 __device__ __forceinline__ int lane_now() {
-  int l;
-  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
-  return l;
+  const uint32_t all = (uint32_t)opaque_uniform(-1);
+  return (int)__builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0));
 }
 // A value that is the same in all lanes, in scalar registers.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
