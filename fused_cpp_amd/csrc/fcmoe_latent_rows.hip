@@ -294,7 +294,8 @@ __global__ __launch_bounds__(kRowThreads) void append_kernel(const Append p) {
   const int64_t page = slot / p.c.page_size, in = slot - page * p.c.page_size;
   if constexpr (E4M3) {
     top = wave_max(top);
-    const float scale = top > 0.0f ? top / kE4M3Max : 1.0f;
+    // 0 for a zero row, and for one of values below the smallest scale: those become zeros
+    const float largest = top / kE4M3Max, scale = largest > 0.0f ? largest : 1.0f;
     if (lane == 0) p.c.scale[page * p.c.scale_page_stride + in] = scale;
 #pragma unroll
     for (int k = 0; k < CPL; ++k) {

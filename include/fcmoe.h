@@ -255,7 +255,7 @@ typedef struct fcmoe_latent_cache {
  * [tokens]: the first latent_dim values RMS-normalised (times weight), the
  * last rot_dim values rotated as above (rot_dim = rope_dim, or with rope_dim 0
  * a multiple of 16 of the latent's last values). An e4m3 row's scale is
- * max|row| / 448 (1 for a zero row). A token whose slot lies outside the cache
+ * max|row| / 448, or 1 where that is 0. A token whose slot lies outside the cache
  * (-1: padding) is not written. Slots of one call must differ: a slot given
  * twice ends up with either row or a mixture. rows_out (optional): [tokens,
  * latent_dim + rope_dim] bf16, the rows before quantisation, for every token. */
