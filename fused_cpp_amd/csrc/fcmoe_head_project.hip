@@ -147,23 +147,26 @@ extern "C" int fcmoe_head_projection(const fcmoe_head_projection_args* a, hipStr
   p.n_tiles = (int)ceil_div(a->n, 16), p.k_chunks = (int)ceil_div(a->k, 32);
   if (ceil_div(a->tokens, 16) * a->heads * p.n_tiles > INT32_MAX)
     return fail(FCMOE_EINVAL, "head_projection: too many tokens");
-  // The largest tile of tokens x channels that still gives every SIMD a wave: a
-  // smaller one reads x and the weights more often, a larger one leaves too few
-  // loads in flight. 128 heads with weights from memory, us: 128 -> 512 at 1
-  // token 7.0, 5.9, 5.6 (64 x 64, 32 x 32, 16 x 16), at 32 8.9, 7.1, 9.2, at 48
-  // 9.7, 11.2 and, 48 x 32, 9.6 (a call alone 8.3, 48 x 64 8.9), at 300 29, 37; 64 x 128 reads x fewer times, little
-  // where K < N: 32, there only past 4096 waves. 512 -> 128 at 48 tokens 18, 12.3,
-  // 12.0, at 100 19, 15, 19 and, 32 x 64, 14, at 300 30, 40 and, 64 x 128, 28.
-  const auto waves = [&](int64_t mt, int64_t nt) { return ceil_div(a->tokens, 16 * mt) * a->heads * ceil_div(p.n_tiles, nt); };
-  if (a->tokens <= 16)
-    head_project_launch<1, 1>(p, stream);
-  else if (a->tokens > 32 && waves(4, 8) >= (a->k < a->n ? 4096 : 640))
+  // The largest tile of tokens x channels that still gives every SIMD a wave (4 a
+  // CU, 256 CUs): a smaller one reads x and the weights more often, a larger one
+  // leaves too few loads in flight. Up to 16 tokens there is one tile of them, up
+  // to 32 one of two, and wider ones would hold rows that are not there. 128 heads,
+  // weights from memory, us for 16 x 16, 32 x 32, 32 x 64, 64 x 64, 64 x 128 (*:
+  // taken): 128 -> 512 at 32 tokens 10.0, 7.2*, 7.9, 8.8, 11.1, at 64 15.7, 12.2,
+  // 10.9, 10.9*, 14.2, at 300 57, 37, 31, 29, 31*, at 2047 377, 257, 208, 184, 162*;
+  // 512 -> 128 at 32 11.3*, 12.6, 13.9, 18, 25, at 128 26, 15.4, 14.2*, 20, 25, at
+  // 300 49, 32, 27, 27*, 25, at 512 82, 49, 40, 33, 30*. Of 787 shapes (64 to 512 values,
+  // 1 to 128 heads, 1 to 4096 tokens) it takes 1.017 of the best tile's time on
+  // average, 1.28 at worst; with 512 waves instead 1.057, with 2048 1.031.
+  constexpr int64_t kSimds = 1024;
+  const auto fills = [&](int64_t mt, int64_t nt) { return ceil_div(a->tokens, 16 * mt) * a->heads * ceil_div(p.n_tiles, nt) >= kSimds; };
+  if (a->tokens > 32 && fills(4, 8))
     head_project_launch<4, 8>(p, stream);
-  else if (a->tokens > 32 && waves(4, 4) >= 1024)
-    a->tokens <= 48 ? head_project_launch<3, 2>(p, stream) : head_project_launch<4, 4>(p, stream);
-  else if (a->tokens > 32 && waves(2, 4) >= 1024)
+  else if (a->tokens > 32 && fills(4, 4))
+    head_project_launch<4, 4>(p, stream);
+  else if (a->tokens > 32 && fills(2, 4))
     head_project_launch<2, 4>(p, stream);
-  else if (waves(2, 2) >= 1024)
+  else if (a->tokens > 16 && fills(2, 2))
     head_project_launch<2, 2>(p, stream);
   else
     head_project_launch<1, 1>(p, stream);
