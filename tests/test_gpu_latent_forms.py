@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from tests import latent_reference as ref
-from tests.test_gpu_latent_attention import BF16, _check_norm_rope, _la, _randn
+from tests.test_gpu_latent_attention import BF16, E4M3, _check_absorbed, _check_norm_rope, _la, _Paged, _queries, _randn
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +60,75 @@ def test_projection_of_one_input_for_all_heads(gpu):
     x = _randn(2, 150, 576).to(BF16)
     assert torch.equal(la.head_projection(x[:, None, :512].expand(-1, 128, -1), w),
                        la.head_projection(x[:, None, :512].expand(-1, 128, -1).contiguous(), w))
+
+
+# ---- norm and rotation, two row groups in flight ------------------------------------------------------------------------
+
+
+def _two_groups(rows, D):
+    """Rows a workgroup takes at a time, and whether it takes two such groups: from 4096 groups up."""
+    lanes = next(n for n in (8, 16, 32, 64) if D // 8 <= n or n == 64)
+    return 256 // lanes, rows >= 256 // lanes * 2 * 2048
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("T,H,D,P", [
+    (131073, 1, 64, 32),    # one row in the last workgroup's first group, none in its second
+    (43700, 3, 48, 48),     # 131100 rows: its second group in part
+    (21850, 3, 128, 64), (10923, 3, 192, 64), (8191, 5, 256, 128), (2731, 6, 512, 64), (5463, 3, 576, 64), (16387, 1, 1024, 64)])
+def test_norm_rope_two_groups(gpu, T, H, D, P, interleaved, in_place):
+    assert _two_groups(T * H, D)[1]
+    x = _randn(T + D, T, H, D, std=3.0).to(BF16)
+    table = ref.rope_table(P, 1000, "cuda")
+    pos = torch.randint(-1, 1000, (T,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(T)).clamp(min=0)
+    w = (1 + 0.2 * _randn(D, D)).to(BF16)
+    for weight, normalize, inverse in ((w, True, False), (None, False, True)):
+        want = _check_norm_rope(x, pos, table, weight, normalize, inverse, interleaved, 1e-6)
+        if in_place:
+            wide = torch.zeros((T, H, D + 8), dtype=BF16, device="cuda")
+            y = wide[..., :D]
+            y.copy_(x)
+            _la().head_norm_rope(y, pos, table, weight=weight, normalize=normalize, inverse=inverse, interleaved=interleaved, out=y)
+            assert torch.equal(y, want) and bool((wide[..., D:] == 0).all())
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_norm_rope_two_groups_one_short(gpu, interleaved):
+    """Just below the limit: one group."""
+    assert not _two_groups(16383, 512)[1] and _two_groups(16384, 512)[1]
+    for T in (16383, 16384):
+        x, pos = _randn(T, T, 1, 512).to(BF16), torch.arange(T, device="cuda") % 50
+        _check_norm_rope(x, pos, ref.rope_table(64, 50, "cuda"), None, True, False, interleaved, 1e-6)
+
+
+# ---- absorbed attention: joining partial results ------------------------------------------------------------------------
+
+
+def _join_form(count, H, n, R, e4m3, cus):
+    """Rows of a group, and whether a strip's partial results are spread over many workgroups."""
+    per = n * H
+    rows = next(r for r in (16, 32, 64, 128) if per <= r or r == 128)
+    groups = count * n * H // rows + count
+    shares = cus // 2 if rows == 128 else cus * (2 if e4m3 and rows == 16 else 1)
+    return rows, min(groups, shares) * (rows // 16) * (R // 4) <= 4096
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("R,P", [(512, 64), (512, 0), (256, 64), (256, 0)])
+@pytest.mark.parametrize("rows,H,n,count,many", [
+    (16, 16, 1, 3, True), (16, 16, 1, 40, False), (16, 5, 3, 150, False),
+    (32, 32, 1, 2, True), (32, 16, 2, 20, False), (64, 64, 1, 1, True), (64, 33, 1, 30, False),
+    (128, 128, 1, 1, True), (128, 128, 1, 33, False), (128, 33, 3, 70, False)])
+def test_absorbed_joins(gpu, rows, H, n, count, many, R, P, e4m3):
+    """Long sequences among short ones, so that groups end up with one, a few and many shares."""
+    assert _join_form(count, H, n, R, e4m3, torch.cuda.get_device_properties(0).multi_processor_count) == (rows, many)
+    lens = [(37 * b) % 300 if b % 4 else 0 for b in range(count)]
+    lens[0], lens[-1] = 9000, 3001
+    pg = _Paged(count, lens, R, P, E4M3 if e4m3 else BF16, page=48)
+    ql, qr = _queries(count, n * count, H, R, P)
+    starts = [n * b for b in range(count + 1)]
+    out, lse = _check_absorbed(pg, lens, ql, qr, starts, 0.07)
+    again = _la().absorbed_attention(ql, qr, pg.cache, pg.table, pg.lens, scale=0.07, return_lse=True,
+                                     query_starts=torch.tensor(starts, dtype=torch.int32, device="cuda"))
+    assert torch.equal(again[0], out) and torch.equal(again[1], lse)
