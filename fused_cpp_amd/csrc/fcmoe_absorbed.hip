@@ -91,8 +91,11 @@ __device__ __forceinline__ int row_groups(const Absorbed& p, const SeqSpan& s, i
 // Tiles of a row group; at least one, so that a sequence without keys still gets its rows written.
 __device__ __forceinline__ int key_tiles(const SeqSpan& s) { return s.len > 0 ? (s.len + kAbsKeys - 1) / kAbsKeys : 1; }
 // Units of a row group: its tiles, and ahead of them what bringing its queries
-// in costs in tiles' time (96 sequences of up to 6000 8-bit keys, 32 rows each:
-// 82 us without it, 70 with).
+// in costs in tiles' time. Times with 0, 1, 3 and 4 of them over those with 2, mean
+// of 104 batches (24 to 300 sequences of up to 300 to 6000 keys, 16 to 512 rows
+// each, bf16 and e4m3, 512 + 64 and 256): 1.14, 1.05, 0.99, 0.99; with 0 each row
+// count and type loses 9 to 29%, with 3 and 4 short batches of 16 rows lose up to 12%
+// and long ones of 128 win as much.
 constexpr int kGroupCost = 2;
 __device__ __forceinline__ int group_units(const SeqSpan& s) { return key_tiles(s) + kGroupCost; }
 
@@ -280,8 +283,8 @@ struct Stager {
     if constexpr (F8) scale = p.c.scale[id * p.c.scale_page_stride + in];
   }
   // The latent row of key u ^ turn (u 0 .. 15, turn 0 or 8) to its place in
-  // buffer `dst`. A CU takes what its L2 lacks at some 10 bytes a clock, what
-  // it has at 60: the two workgroups that share keys bring the halves of their
+  // buffer `dst`. What its L2 lacks comes to a CU at some 10 bytes a clock
+  // (4.9 TB/s over 256 CUs), what it has several times as fast: the two workgroups that share keys bring the halves of their
   // 16 in opposite orders, so that each finds one half fetched by the other.
   __device__ __forceinline__ void load(lds_u8* dst, int u) const {
     const uint32_t ln = (uint32_t)lane_now();
@@ -339,9 +342,10 @@ __device__ __forceinline__ v4f lds_v4f(const lds_u8* p) { return *(const __attri
 // take all of a SIMD's 512 for its one wave. Half of those are accumulation
 // registers, which MFMAs can read as operands; Q lies there, and its MFMAs are
 // written out, because the compiler would copy each fragment to an ordinary
-// register first (a tile of 64 rows took 10000 clocks, with that 6900, now
-// 6300; its products alone 2200). With eight
-// waves instead, Q leaves no registers to read K fragments ahead with (9200).
+// register first. With eight waves instead, Q would leave no registers to read K
+// fragments ahead with. A tile of 64 rows takes 6100 clocks: 2200 for S, 800 for the
+// weights and their barrier, 2300 for P V, the rest for the next tile's addresses
+// and arrival; its products alone are 2200 (128 heads, 64 sequences of 4096 bf16 rows).
 //
 // PAIR: the rows of a sequence fill two workgroups (65 rows and more); these
 // two take the same tiles at the same time on the same XCD, whose L2 then
@@ -514,7 +518,7 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
       }
     } else {
       // Through LDS, laid out as a bf16 tile: read straight into fragments, each
-      // wave would fetch every row in 64-byte pieces (15000 clocks for 64 rows).
+      // wave would fetch every row in 64-byte pieces.
       // 16-bit tiles: in the second buffer, which the first iteration fills only
       // once everyone has met at its barrier.
       constexpr int QR = ROWS / 4;  // rows a wave brings
@@ -620,7 +624,7 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
       };
       v4f s[MT];
       // with either kind and without the next tile's loads, as straight-line code
-      // each: a branch around every load costs a wave 30 clocks
+      // each: no branch around every load
       auto scores = [&](auto loads_) {
         constexpr int LOADS = decltype(loads_)::value;
         static_assert(STEPS == Stager<R, P, F8>::WLOADS + Stager<R, P, F8>::WRLOADS, "a load a step");
@@ -702,6 +706,11 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
         grown = grown || (top[r] - m[r]) * c2 > 8.0f;
       }
       if (__any(grown)) *(lds_i32*)(lds + FLAGS + 4 * buf) = 1;  // every lane writes the same
+      // The weights go into P V as bf16, off by at most 2^-8 of themselves: a product's operands are of one type, and a
+      // second part of each would double the products. An 8-bit cache's scales, which differ by token, go into them first.
+      // The sum is of what they were before (of the rounded ones it would leave the output's error as it is, and lse worse):
+      // outputs err by 0.0020 to 0.0023 of their size against 64 bits (root mean square), where rounding the output alone
+      // leaves 0.0017.
       float sum[MT];
       auto weights = [&]() {
         const int wl = lane_now(), wq = wl / 16, wc = wl % 16;

@@ -17,15 +17,16 @@
 // Two kernels:
 //
 // narrow: 128 rows, 32 a wave, two workgroups a CU, whose waves fill each
-//   other's waits. What one has before its first tile and behind its last is
-//   hidden by the other; a tile of both takes each SIMD 2560 clocks of products
-//   and some 5500 in all.
+//   other's waits. What one has before its first tile and behind its last (some
+//   8000 and 2000 clocks) is hidden by the other as far as that has tiles left; a
+//   tile of one takes some 5000 clocks, in which each SIMD has 2560 of products
+//   for the two.
 // wide: 256 rows, 64 a wave, one workgroup a CU: every fragment read from LDS
 //   feeds two products, and the exponentials of one tile stand between the
-//   products of the next, written out in that order (a tile 2760 clocks, of them
-//   2560 of products). 16384 tokens, 16 heads: 1115 us against 1400, 1.23 PFLOP/s
-//   of what causality leaves; the card lowers its clock at this load, as for a
-//   large matrix product (1.23 to 1.5 PFLOP/s).
+//   products of the next, written out in that order. 16384 tokens, 16 heads: 1120
+//   us against 1400, 1.23 PFLOP/s of what causality leaves (large matrix products
+//   reach 1.23 to 1.5); the matrix units are busy 0.65 of the launch's clocks, masked
+//   tiles and the ends of row blocks included.
 #include <type_traits>
 
 #include "fcmoe_internal.h"
@@ -239,6 +240,9 @@ __global__ __launch_bounds__(kExpWaves * kWave, 2) void expanded_narrow_kernel(c
         for (int i = 0; i < 16; ++i) o[t][i] *= a;
     }
     const float mc = m == -INFINITY ? 0.0f : m * c2;
+    // The weights go into P V as bf16, off by at most 2^-8 of themselves: a product's operands are of one type, and a second
+    // part of each would double the products. Their sum is of what they were before (of the rounded ones it would leave the
+    // output's error as it is, and lse worse).
     v8bf pf[4];
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
@@ -601,6 +605,7 @@ __global__ __launch_bounds__(kExpWaves * kWave, 1) void expanded_wide_kernel(con
       vlo[n % (vAhead + 1)] = read_tr16(vb + (va ^ (tt << 6)) + 16 * st * 2 * V);
       vhi[n % (vAhead + 1)] = read_tr16(vb + (va ^ ((TO == 4 ? tt ^ 2 : tt) << 6)) + (16 * st + 8) * 2 * V);
     };
+    // The weights rounded to bf16 for P V and summed before that, as in the other form.
     auto finish = [&](int g) {  // group g: row tile g / 8, key half (g % 8) / 4, registers 4 (g % 4) ..
       const float* w = e[g & 1];
       sum[g / 8][0] += w[0] + w[1];
@@ -773,7 +778,9 @@ __global__ __launch_bounds__(kExpWaves * kWave) void expanded_combine_kernel(con
 // Rows of a row block. 256 make two products of each K and V fragment read from
 // LDS but leave a workgroup alone on its CU, with what comes before its first
 // tile and behind its last in the open: it pays from some 16 tiles a row on
-// average. Measured wide against narrow, 128 + 64 / 128: 128 heads of 1500
+// average. The averages are over the batch: lengths are on the device, so one
+// long prompt among many short ones takes the form that the short ones ask for.
+// Measured wide against narrow, 128 + 64 / 128: 128 heads of 1500
 // tokens 132 us, 129, of 2048 210, 225; 16 heads of 4 x 4096 188, 200; 160 tokens
 // behind 8000, 128 heads, 191, 244; but 32 x 128 tokens, 128 heads, 167, 82.
 int expanded_rows(const fcmoe_expanded_args* a) {

@@ -115,11 +115,6 @@ __device__ __forceinline__ float other_half(float v) {
 }
 
 // A value the compiler cannot see through: what depends on it is formed after this point.
-__device__ __forceinline__ int opaque(int v) {
-  asm volatile("" : "+v"(v));
-  return v;
-}
-
 __device__ __forceinline__ int64_t opaque_uniform(int64_t v) {
   asm volatile("" : "+s"(v));
   return v;

@@ -20,14 +20,16 @@ values, ``rope_dim`` rotated key values beside them) lies in a paged cache:
     rows = latent_cache_append(..., return_rows=True)
     values = expanded_attention(q, kv_up, rows[:, latent_dim:], query_starts, scale=...)
 
-Everything is bf16 in and out with fp32 arithmetic; the cache is bf16, or e4m3
-with one fp32 scale a token. Inference only: inputs that require a gradient are
-refused while gradients are recorded, and inputs with a forward-mode tangent;
-an ``out`` or a cache that is written counts as changed in place. Calls run on the current stream of their
-tensors' device, allocate through torch, read lengths, positions, slots and
-page ids on the device only, and can be captured into a HIP graph. What a call
-writes may lie between the rows of what it reads, as views of one tensor do,
-but share no memory with it.
+Everything is bf16 in and out. Norms, rotations, scores, softmax sums and all
+accumulators are fp32; the attentions round each softmax weight once to bf16 for
+its product with the values (times its token's scale in an e4m3 cache). The cache
+is bf16, or e4m3 with one fp32 scale a token. Inference only: inputs that require
+a gradient are refused while gradients are recorded, and inputs with a forward-mode
+tangent; an ``out`` or a cache that is written counts as changed in place. Calls
+run on the current stream of their tensors' device, allocate through torch, read
+lengths, positions, slots and page ids on the device only, and can be captured into
+a HIP graph. What a call writes may lie between the rows of what it reads, as views
+of one tensor do, but share no memory with it.
 """
 
 from __future__ import annotations

@@ -208,7 +208,10 @@ int fcmoe_i8gemm_pair(const uint16_t* x, int64_t m, int64_t k, const void* w1_pa
  * The steps between the W8A8 projections of a DeepSeek latent-attention layer:
  * what the reference's adapter leaves to its caller's attention backend. No
  * counterpart in the fused-MoE reference path. All tensors are bf16 unless
- * stated; strides are in elements, the last dimension is contiguous. What a
+ * stated; strides are in elements, the last dimension is contiguous. Sums,
+ * norms, scores and accumulators are binary32; the attentions round each softmax
+ * weight (times its token's scale in an e4m3 cache) once to bf16 for its product
+ * with the values. What a
  * call writes shares no memory with what it reads. */
 
 /* Per-head RMS norm and position rotation of x [tokens, heads, dim], one pass:
