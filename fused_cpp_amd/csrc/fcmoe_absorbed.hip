@@ -1076,7 +1076,7 @@ void combine_launch(const Absorbed& p, const AbsPlan& pl, hipStream_t stream) {
 int check_absorbed(const fcmoe_absorbed_args* a) {
   if (!a) return fail(FCMOE_EINVAL, "absorbed_attention: NULL args");
   if (const int rc = check_latent_cache(a->cache, "absorbed_attention")) return rc;
-  if (a->tokens < 0 || a->batch <= 0 || a->batch > (1 << 20) || a->heads <= 0 || a->heads > 65536 ||
+  if (a->tokens < 0 || a->tokens > INT32_MAX || a->batch <= 0 || a->batch > (1 << 20) || a->heads <= 0 || a->heads > 65536 ||
       a->tokens * a->heads > INT32_MAX / 2 || a->table_width < 0 || a->table_width > INT32_MAX ||
       a->page_table_stride < 0)
     return fail(FCMOE_EINVAL, "absorbed_attention: bad shape");

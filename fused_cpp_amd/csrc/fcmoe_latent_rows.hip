@@ -375,8 +375,8 @@ extern "C" int fcmoe_head_norm_rope(const fcmoe_head_norm_rope_args* a, hipStrea
   NormRope p{};
   p.x = a->x, p.out = a->out;
   p.xt = a->x_token_stride, p.xh = a->x_head_stride, p.ot = a->out_token_stride, p.oh = a->out_head_stride;
+  if (a->tokens > INT32_MAX || a->tokens * a->heads / 4 > INT32_MAX) return fail(FCMOE_EINVAL, "head_norm_rope: too many rows");
   p.rows = a->tokens * a->heads;
-  if (a->tokens > INT32_MAX || p.rows / 4 > INT32_MAX) return fail(FCMOE_EINVAL, "head_norm_rope: too many rows");
   p.heads = (int)a->heads, p.D = (int)a->dim, p.P = (int)a->rope_dim;
   p.positions = a->positions, p.pos_i64 = a->positions_i64;
   p.table = a->cos_sin, p.table_rows = a->table_rows;
