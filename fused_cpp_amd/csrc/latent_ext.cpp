@@ -138,33 +138,51 @@ class Reach {
   int64_t left_ = 0;
 };
 
-int64_t address(const at::Tensor& t) { return (int64_t)reinterpret_cast<uintptr_t>(t.data_ptr()); }
 int64_t byte_stride(const at::Tensor& t, int64_t d) { return t.stride(d) * (int64_t)t.element_size(); }
-// Bytes from the first to behind the last.
-int64_t extent(const at::Tensor& t) {
-  int64_t e = (int64_t)t.element_size();
-  for (int64_t d = 0; d < t.dim(); ++d) e += (t.size(d) - 1) * byte_stride(t, d);
-  return e;
-}
 
-bool share_memory(const at::Tensor& a, const at::Tensor& b) {
-  if (!a.defined() || !b.defined() || a.device() != b.device() || a.numel() == 0 || b.numel() == 0) return false;
-  const int64_t at_a = address(a), at_b = address(b);
-  if (at_a + extent(a) <= at_b || at_b + extent(b) <= at_a) return false;
+// A tensor's bytes, from the first to behind the last: none of one that is undefined or empty.
+struct Place {
+  const at::Tensor* t;
+  int64_t begin = 0, end = 0;
+  explicit Place(const at::Tensor& tensor) : t(&tensor) {
+    if (!t->defined() || t->numel() == 0) return;
+    const at::IntArrayRef sizes = t->sizes(), strides = t->strides();
+    int64_t last = 0;
+    for (size_t d = 0; d < sizes.size(); ++d) last += (sizes[d] - 1) * strides[d];
+    begin = (int64_t)reinterpret_cast<uintptr_t>(t->const_data_ptr());
+    end = begin + (last + 1) * (int64_t)t->element_size();
+  }
+};
+
+bool share_memory(const Place& pa, const Place& pb) {
+  if (pa.end <= pb.begin || pb.end <= pa.begin) return false;
+  const at::Tensor &a = *pa.t, &b = *pb.t;
+  if (a.device() != b.device()) return false;
   Reach r;
   for (int64_t d = 0; d < a.dim(); ++d) r.add(byte_stride(a, d), -(a.size(d) - 1), 0);
   for (int64_t d = 0; d < b.dim(); ++d) r.add(byte_stride(b, d), 0, b.size(d) - 1);
   r.add(1, -((int64_t)a.element_size() - 1), (int64_t)b.element_size() - 1);
-  return r.zero(at_b - at_a);
+  return r.zero(pb.begin - pa.begin);
 }
 
 // Whether two places of a tensor are one: two index vectors that differ first
 // in dimension `d` (by 1 and more; the others by anything) and meet.
 bool shares_itself(const at::Tensor& t) {
   if (t.numel() < 2) return false;
+  const at::IntArrayRef sizes = t.sizes(), strides = t.strides();
+  // Nearly all tensors' dimensions lie inside one another in their order: each
+  // stride is beyond all that the ones behind it reach.
+  int64_t reach = 0;
+  bool nested = true;
+  for (size_t d = sizes.size(); d-- > 0;) {
+    if (sizes[d] < 2) continue;
+    nested = nested && strides[d] > reach;
+    reach += (sizes[d] - 1) * strides[d];
+  }
+  if (nested) return false;
   for (int64_t d = 0; d < t.dim(); ++d) {
-    if (t.size(d) < 2) continue;
-    if (t.stride(d) == 0) return true;
+    if (sizes[d] < 2) continue;
+    if (strides[d] == 0) return true;
     Reach r;
     for (int64_t e = d + 1; e < t.dim(); ++e) r.add(byte_stride(t, e), -(t.size(e) - 1), t.size(e) - 1);
     r.add(byte_stride(t, d), 0, t.size(d) - 2);
@@ -173,13 +191,26 @@ bool shares_itself(const at::Tensor& t) {
   return false;
 }
 
-// What a call writes lies apart from what it reads, and no two of its places are one.
-void check_written(const at::Tensor& written, const char* name, std::initializer_list<const at::Tensor*> others,
-                   const char* what) {
-  if (!written.defined()) return;
-  TORCH_CHECK(!shares_itself(written), what, ": ", name, " must not overlap itself");
-  for (const at::Tensor* t : others)
-    TORCH_CHECK(!share_memory(written, *t), what, ": ", name, " must not overlap the call's other tensors");
+// What a call writes lies apart from what it reads and from what else it
+// writes, and no two places of it are one.
+struct Written {
+  const at::Tensor* t;
+  const char* name;
+};
+void check_written(std::initializer_list<Written> written, std::initializer_list<const at::Tensor*> read, const char* what) {
+  c10::SmallVector<Place, 4> mine;
+  for (const Written& w : written) {
+    if (w.t->defined()) TORCH_CHECK(!shares_itself(*w.t), what, ": ", w.name, " must not overlap itself");
+    mine.emplace_back(*w.t);
+  }
+  for (size_t i = 0; i < mine.size(); ++i)
+    for (size_t j = 0; j < i; ++j)
+      TORCH_CHECK(!share_memory(mine[i], mine[j]), what, ": ", written.begin()[i].name, " must not overlap ", written.begin()[j].name);
+  for (const at::Tensor* t : read) {
+    const Place p(*t);
+    for (size_t i = 0; i < mine.size(); ++i)
+      TORCH_CHECK(!share_memory(mine[i], p), what, ": ", written.begin()[i].name, " must not overlap the call's inputs");
+  }
 }
 
 // A caller's output, or a new one. `direct` is what the kernel writes: the
@@ -253,7 +284,8 @@ at::Tensor head_norm_rope(at::Tensor x, at::Tensor positions, at::Tensor cos_sin
   const bool in_place = given.defined() && given.data_ptr() == x.data_ptr() && stride_at(given, 0) == stride_at(x, 0) &&
                         stride_at(given, 1) == stride_at(x, 1) && stride_at(given, 2) == stride_at(x, 2);
   const at::Tensor none;
-  check_written(given, "out (unless it is x itself)", {in_place ? &none : &x, &positions, &cos_sin, &w}, what);
+  if (given.defined())
+    check_written({{&given, "out (unless it is x itself)"}}, {in_place ? &none : &x, &positions, &cos_sin, &w}, what);
   check_devices(x, {&positions, &cos_sin, &w, &given}, what);
   c10::DeviceGuard guard(x.device());
   Out o = output(out, x.sizes(), x, 1, what);
@@ -348,9 +380,8 @@ OptTensor latent_cache_append(at::Tensor kv, at::Tensor positions, at::Tensor sl
                       w.sizes());
   }
   check_no_grad({&kv, &cos_sin, &w, &latent, &rope, &scale}, what);
-  check_written(latent, "cache.latent", {&rope, &scale, &kv, &positions, &slots, &cos_sin, &w}, what);
-  check_written(rope, "cache.rope", {&scale, &kv, &positions, &slots, &cos_sin, &w}, what);
-  check_written(scale, "cache.scale", {&kv, &positions, &slots, &cos_sin, &w}, what);
+  check_written({{&latent, "cache.latent"}, {&rope, "cache.rope"}, {&scale, "cache.scale"}},
+                {&kv, &positions, &slots, &cos_sin, &w}, what);
   check_devices(kv, {&positions, &slots, &cos_sin, &latent, &rope, &scale, &w}, what);
   c10::DeviceGuard guard(kv.device());
   OptTensor rows;
@@ -405,7 +436,7 @@ at::Tensor head_projection(at::Tensor x, at::Tensor packed, int64_t heads, int64
   check_output(out, {T, heads, n}, what);
   const at::Tensor given = opt(out);
   check_no_grad({&x}, what);
-  check_written(given, "out", {&x, &packed}, what);
+  if (given.defined()) check_written({{&given, "out"}}, {&x, &packed}, what);
   check_devices(x, {&packed, &given}, what);
   c10::DeviceGuard guard(x.device());
   Out o = output(out, {T, heads, n}, x, 4, what);
@@ -471,7 +502,9 @@ std::tuple<at::Tensor, OptTensor> absorbed_attention(at::Tensor q_latent, OptTen
   check_output(out, {T, H, R}, what);
   const at::Tensor given = opt(out);
   check_no_grad({&q_latent, &q_rope, &latent, &rope, &cache_scale}, what);
-  check_written(given, "out", {&q_latent, &q_rope, &latent, &rope, &cache_scale, &page_table, &kv_lens, &starts}, what);
+  if (given.defined())
+    check_written({{&given, "out"}}, {&q_latent, &q_rope, &latent, &rope, &cache_scale, &page_table, &kv_lens, &starts},
+                  what);
   check_devices(q_latent, {&q_rope, &latent, &rope, &cache_scale, &page_table, &kv_lens, &starts, &given}, what);
   c10::DeviceGuard guard(q_latent.device());
   Out o = output(out, {T, H, R}, q_latent, 4, what);
@@ -541,7 +574,7 @@ std::tuple<at::Tensor, OptTensor> expanded_attention(at::Tensor q, at::Tensor kv
   check_output(out, {T, H, V}, what);
   const at::Tensor given = opt(out);
   check_no_grad({&q, &kv, &k_rope}, what);
-  check_written(given, "out", {&q, &kv, &k_rope, &query_starts, &kv_starts}, what);
+  if (given.defined()) check_written({{&given, "out"}}, {&q, &kv, &k_rope, &query_starts, &kv_starts}, what);
   check_devices(q, {&kv, &k_rope, &query_starts, &kv_starts, &given}, what);
   c10::DeviceGuard guard(q.device());
   Out o = output(out, {T, H, V}, q, 4, what);
