@@ -1057,11 +1057,19 @@ void combine_launch(const Absorbed& p, const AbsPlan& pl, hipStream_t stream) {
   auto go = [&](auto rows_) {
     constexpr int ROWS = decltype(rows_)::value;
     const int64_t strips = (pl.by_group ? pl.groups : pl.shares) * (ROWS / 16);
-    // few strips: their partials are spread over more workgroups
-    if (strips * (R / 4) <= 4096)
-      hipLaunchKernelGGL((absorbed_combine_many_kernel<R, ROWS>), dim3((unsigned)strips, R / 4), dim3(1024), 0, stream, p);
-    else
-      hipLaunchKernelGGL((absorbed_combine_kernel<R, ROWS>), dim3((unsigned)strips, R / 64), dim3(256), 0, stream, p);
+    // Few strips: their partials are spread over more workgroups, of 16 waves each, which pays while there are no more than
+    // two a CU. Attention and join, us, spread and not: 16 rows, 512 + 64, 256 workgroups (one sequence of 60000) 25.0,
+    // 44.0, 512 (two of 30000) 27.9, 33.7, 1024 (four of 15000) 32.9, 27.7, 4096 (16 of 4000) 61, 24; 32 rows 512 32.2, 48.4,
+    // 1024 37.5, 36.1; 64 rows 1024 44.9, 52.9, 2048 54, 41; latent 256 16 rows 512 21.4, 22.5, 1024 26.5, 19.9, 128 rows
+    // 1024 43.9, 42.7.
+    constexpr int64_t kSpread = 512;
+    if constexpr (ROWS / 16 * (R / 4) <= kSpread) {  // one group's
+      if (strips * (R / 4) <= kSpread) {
+        hipLaunchKernelGGL((absorbed_combine_many_kernel<R, ROWS>), dim3((unsigned)strips, R / 4), dim3(1024), 0, stream, p);
+        return;
+      }
+    }
+    hipLaunchKernelGGL((absorbed_combine_kernel<R, ROWS>), dim3((unsigned)strips, R / 64), dim3(256), 0, stream, p);
   };
   if (pl.rows == 128)
     go(std::integral_constant<int, 128>{});

@@ -111,20 +111,22 @@ def _join_form(count, H, n, R, e4m3, cus):
     rows = next(r for r in (16, 32, 64, 128) if per <= r or r == 128)
     groups = count * n * H // rows + count
     shares = cus // 2 if rows == 128 else cus * (2 if e4m3 and rows == 16 else 1)
-    return rows, min(groups, shares) * (rows // 16) * (R // 4) <= 4096
+    return rows, min(groups, shares) * (rows // 16) * (R // 4) <= 512
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("R,P", [(512, 64), (512, 0), (256, 64), (256, 0)])
-@pytest.mark.parametrize("rows,H,n,count,many", [
-    (16, 16, 1, 3, True), (16, 16, 1, 40, False), (16, 5, 3, 150, False),
-    (32, 32, 1, 2, True), (32, 16, 2, 20, False), (64, 64, 1, 1, True), (64, 33, 1, 30, False),
-    (128, 128, 1, 1, True), (128, 128, 1, 33, False), (128, 33, 3, 70, False)])
-def test_absorbed_joins(gpu, rows, H, n, count, many, R, P, e4m3):
+@pytest.mark.parametrize("rows,H,n,count,spread_from", [
+    (16, 16, 1, 1, 512), (16, 16, 1, 2, 512), (16, 9, 1, 4, 256), (16, 16, 1, 3, 256), (16, 16, 1, 40, 0), (16, 5, 3, 150, 0),
+    (32, 32, 1, 1, 512), (32, 17, 1, 1, 512), (32, 32, 1, 2, 256), (32, 16, 2, 20, 0),
+    (64, 33, 1, 1, 512), (64, 64, 1, 1, 256), (64, 33, 1, 30, 0),
+    (128, 65, 1, 1, 256), (128, 128, 1, 1, 0), (128, 128, 1, 33, 0), (128, 33, 3, 70, 0)])
+def test_absorbed_joins(gpu, rows, H, n, count, spread_from, R, P, e4m3):
     """Long sequences among short ones, so that groups end up with one, a few and many shares."""
-    assert _join_form(count, H, n, R, e4m3, torch.cuda.get_device_properties(0).multi_processor_count) == (rows, many)
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    assert _join_form(count, H, n, R, e4m3, cus) == (rows, R <= spread_from)  # latent widths whose joins are spread
     lens = [(37 * b) % 300 if b % 4 else 0 for b in range(count)]
-    lens[0], lens[-1] = 9000, 3001
+    lens[-1], lens[0] = 3001, 9000
     pg = _Paged(count, lens, R, P, E4M3 if e4m3 else BF16, page=48)
     ql, qr = _queries(count, n * count, H, R, P)
     starts = [n * b for b in range(count + 1)]
