@@ -92,7 +92,7 @@ struct NormRope {
 // LPR lanes hold one row, CPL chunks of 8 values each. A workgroup takes
 // 256 / LPR rows at a time and RPT such groups, all of whose loads are issued
 // before the first is used (a row is a short dependent chain: load, reduce,
-// store; one row per lane group in flight left the memory pipe idle).
+// store).
 template <int LPR, int CPL, int RPT>
 __global__ __launch_bounds__(kRowThreads) void norm_rope_kernel(const NormRope p) {
   constexpr int RPG = kRowThreads / LPR;  // rows of a group
@@ -210,9 +210,11 @@ __global__ __launch_bounds__(kRowThreads) void norm_rope_any_kernel(const NormRo
 template <int LPR, int CPL>
 void norm_rope_launch(const NormRope& p, hipStream_t stream) {
   constexpr int RPG = kRowThreads / LPR;
-  // Two row groups in flight once they still leave a workgroup for every CU
-  // slot; below that one group each spreads the rows further.
-  if (p.rows >= (int64_t)RPG * 2 * 2048) {
+  // Two row groups in flight once the workgroups go round many times; below
+  // that one group each spreads the rows further. One and two, us: rows of 512
+  // 8192 groups 18.0, 18.9, 16384 33.5, 34.9, 32768 62.8, 61.0, 65536 122.8,
+  // 117.8; of 192 16384 31.4, 32.2, 32768 61.2, 59.1; of 1024 32768 95.4, 95.3.
+  if (p.rows >= (int64_t)RPG * 32768) {
     hipLaunchKernelGGL((norm_rope_kernel<LPR, CPL, 2>), dim3((unsigned)ceil_div(p.rows, RPG * 2)), dim3(kRowThreads),
                        0, stream, p);
   } else {

@@ -66,17 +66,17 @@ def test_projection_of_one_input_for_all_heads(gpu):
 
 
 def _two_groups(rows, D):
-    """Rows a workgroup takes at a time, and whether it takes two such groups: from 4096 groups up."""
+    """Rows a workgroup takes at a time, and whether it takes two such groups: from 32768 groups up."""
     lanes = next(n for n in (8, 16, 32, 64) if D // 8 <= n or n == 64)
-    return 256 // lanes, rows >= 256 // lanes * 2 * 2048
+    return 256 // lanes, rows >= 256 // lanes * 32768
 
 
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("interleaved", [True, False])
 @pytest.mark.parametrize("T,H,D,P", [
-    (131073, 1, 64, 32),    # one row in the last workgroup's first group, none in its second
-    (43700, 3, 48, 48),     # 131100 rows: its second group in part
-    (21850, 3, 128, 64), (10923, 3, 192, 64), (8191, 5, 256, 128), (2731, 6, 512, 64), (5463, 3, 576, 64), (16387, 1, 1024, 64)])
+    (1048577, 1, 64, 32),   # one row in the last workgroup's first group, none in its second
+    (349540, 3, 48, 48),    # 1048620 rows: its second group in part
+    (174770, 3, 128, 64), (87385, 3, 192, 64), (52431, 5, 256, 128), (21847, 6, 512, 64), (43691, 3, 576, 64), (131075, 1, 1024, 64)])
 def test_norm_rope_two_groups(gpu, T, H, D, P, interleaved, in_place):
     assert _two_groups(T * H, D)[1]
     x = _randn(T + D, T, H, D, std=3.0).to(BF16)
@@ -96,8 +96,8 @@ def test_norm_rope_two_groups(gpu, T, H, D, P, interleaved, in_place):
 @pytest.mark.parametrize("interleaved", [True, False])
 def test_norm_rope_two_groups_one_short(gpu, interleaved):
     """Just below the limit: one group."""
-    assert not _two_groups(16383, 512)[1] and _two_groups(16384, 512)[1]
-    for T in (16383, 16384):
+    assert not _two_groups(131071, 512)[1] and _two_groups(131072, 512)[1]
+    for T in (131071, 131072):
         x, pos = _randn(T, T, 1, 512).to(BF16), torch.arange(T, device="cuda") % 50
         _check_norm_rope(x, pos, ref.rope_table(64, 50, "cuda"), None, True, False, interleaved, 1e-6)
 
