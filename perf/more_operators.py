@@ -1,5 +1,6 @@
-"""The measured work of ``fused_cpp_amd.latent_attention`` beyond plain causal attention: what serving long contexts
-and drafted tokens over a latent cache needs, each through its public entry point.
+"""The measured work of ``fused_cpp_amd.latent_attention`` beyond plain causal attention and of
+``fused_cpp_amd.latent_context``: what serving long contexts and drafted tokens over a latent cache needs, each through
+its public entry point.
 
 A case is a dict of plain values with an ``op``:
 
@@ -269,6 +270,7 @@ def prepare(case, seed):
 
 def _run_own(st):
     from fused_cpp_amd import latent_attention as la
+    from fused_cpp_amd import latent_context as lc
 
     case = st["case"]
     op = case["op"]
@@ -277,7 +279,7 @@ def _run_own(st):
                                      scale=st["sm"], window=case["window"], sinks=case["sinks"],
                                      return_lse=case["lse"])
     if op == "heaviest":
-        return la.heaviest_positions(st["weights"], st["lens"], case["keep"], sinks=case["sinks"],
+        return lc.heaviest_positions(st["weights"], st["lens"], case["keep"], sinks=case["sinks"],
                                      recent=case["recent"])
     cache = la.LatentCache(st["latent"], st["rope"], st["scale"])
     if op == "window":
@@ -285,15 +287,15 @@ def _run_own(st):
                                      query_starts=st["starts"] if case["n"] > 1 else None, window=case["window"],
                                      sinks=case["sinks"], return_lse=case["lse"])
     if op == "tree":
-        tree = la.draft_tree(st["parents"], st["starts"], case["nodes"])
+        tree = lc.draft_tree(st["parents"], st["starts"], case["nodes"])
         got = la.absorbed_attention(st["q_latent"], st["q_rope"], cache, st["table"], st["lens"], scale=st["sm"],
                                     query_starts=st["starts"], tree=tree, return_lse=case["lse"])
         return (*(got if case["lse"] else (got,)), tree.masks, tree.depths)
     if op == "weights":
-        return la.attention_weights(st["q_latent"], st["q_rope"], cache, st["table"], st["lens"], st["lse"],
+        return lc.attention_weights(st["q_latent"], st["q_rope"], cache, st["table"], st["lens"], st["lse"],
                                     scale=st["sm"], query_starts=st["starts"] if case["n"] > 1 else None,
                                     previous=st["previous"])
-    la.latent_cache_move(cache, st["table"], st["positions"], st["counts"], to_table=st["to_table"],
+    lc.latent_cache_move(cache, st["table"], st["positions"], st["counts"], to_table=st["to_table"],
                          starts=st["first"] if case["drafts"] else None)
     return [t for t in (st["latent"], st["rope"], st["scale"]) if t is not None]
 
@@ -516,7 +518,8 @@ def exact(case, seed):
     st = prepare(case, seed)
     f64 = torch.float64
     new, kv = st["new"], st["kv_lens"]
-    if w > 1e12 or sum(n * L for n, L in zip(new, kv)) * case["H"] * (st["q"] if op == "prompt" else st["q_latent"]).shape[-1] > 2e12:
+    pairs = sum(n * L for n, L in zip(new, kv)) * case["H"]
+    if w > 1e12 or pairs * (case["N"] if op == "prompt" else case["R"]) > 2e12:
         return None
     total = st["previous"].to(f64) if op == "weights" else None
     outs, lses = [], []
