@@ -33,7 +33,8 @@ ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 ARCH = os.environ.get("FCMOE_OFFLOAD_ARCH", "gfx950")
 
 HIP_SOURCES = ["fcmoe_api.hip", "fcmoe_route.hip", "fcmoe_quant.hip", "fcmoe_gemm.hip", "fcmoe_gemm_lds.hip", "fcmoe_gemm_smallm.hip", "fcmoe_gemm_mid.hip", "fcmoe_combine.hip", "fcmoe_decode_tail.hip", "fcmoe_decode_bf16.hip", "fcmoe_router.hip", "fcmoe_latent_rows.hip",
-               "fcmoe_head_project.hip", "fcmoe_absorbed.hip", "fcmoe_expanded.hip"]
+               "fcmoe_head_project.hip", "fcmoe_absorbed.hip", "fcmoe_expanded.hip", "fcmoe_absorbed_masked.hip",
+               "fcmoe_expanded_window.hip", "fcmoe_weights.hip", "fcmoe_latent_select.hip"]
 # bench-only measurement probes: a library of their own (fcmoe_probe.h), linked against libfcmoe.so
 PROBE_SOURCES = ["fcmoe_probe.hip"]
 EXT_SOURCES = ["moe_ext.cpp", "latent_ext.cpp"]

@@ -137,6 +137,42 @@ class ExpandedArgs(ctypes.Structure):
     ]
 
 
+class KeyMask(ctypes.Structure):
+    """Mirror of ``struct fcmoe_key_mask``."""
+
+    _fields_ = [
+        ("window", _I64), ("sinks", _I64),
+        ("tree_masks", _P), ("mask_words", _I64), ("mask_stride", _I64), ("tree_depths", _P),
+    ]
+
+
+class AttentionWeightsArgs(ctypes.Structure):
+    """Mirror of ``struct fcmoe_attention_weights_args``."""
+
+    _fields_ = [
+        ("q_latent", _P), ("q_rope", _P), ("tokens", _I64), ("heads", _I64), ("batch", _I64),
+        ("q_latent_token_stride", _I64), ("q_latent_head_stride", _I64),
+        ("q_rope_token_stride", _I64), ("q_rope_head_stride", _I64),
+        ("cache", LatentCacheDesc),
+        ("page_table", _P), ("table_width", _I64), ("page_table_stride", _I64),
+        ("kv_lens", _P), ("query_starts", _P), ("lse", _P), ("scale", ctypes.c_float),
+        ("previous", _P), ("previous_stride", _I64), ("out", _P), ("out_stride", _I64), ("positions", _I64),
+        ("workspace", _P), ("workspace_bytes", _SZ),
+    ]
+
+
+class LatentMoveArgs(ctypes.Structure):
+    """Mirror of ``struct fcmoe_latent_move_args``."""
+
+    _fields_ = [
+        ("cache", LatentCacheDesc),
+        ("page_table", _P), ("table_width", _I64), ("page_table_stride", _I64),
+        ("to_table", _P), ("to_width", _I64), ("to_stride", _I64),
+        ("positions", _P), ("most", _I64), ("positions_stride", _I64),
+        ("counts", _P), ("starts", _P), ("batch", _I64),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/fcmoe.h.
 SIGNATURES = {
     "fcmoe_last_error": (ctypes.c_char_p, []),
@@ -173,6 +209,15 @@ SIGNATURES = {
     "fcmoe_absorbed_attention": (_I, [ctypes.POINTER(AbsorbedArgs), _P]),
     "fcmoe_expanded_attention_workspace_bytes": (_SZ, [ctypes.POINTER(ExpandedArgs)]),
     "fcmoe_expanded_attention": (_I, [ctypes.POINTER(ExpandedArgs), _P]),
+    "fcmoe_absorbed_attention_masked_workspace_bytes": (_SZ, [ctypes.POINTER(AbsorbedArgs), ctypes.POINTER(KeyMask)]),
+    "fcmoe_absorbed_attention_masked": (_I, [ctypes.POINTER(AbsorbedArgs), ctypes.POINTER(KeyMask), _P]),
+    "fcmoe_expanded_attention_masked_workspace_bytes": (_SZ, [ctypes.POINTER(ExpandedArgs), ctypes.POINTER(KeyMask)]),
+    "fcmoe_expanded_attention_masked": (_I, [ctypes.POINTER(ExpandedArgs), ctypes.POINTER(KeyMask), _P]),
+    "fcmoe_draft_tree": (_I, [_P, _I64, _P, _I64, _I64, _P, _P, _P]),
+    "fcmoe_attention_weights_workspace_bytes": (_SZ, [ctypes.POINTER(AttentionWeightsArgs)]),
+    "fcmoe_attention_weights": (_I, [ctypes.POINTER(AttentionWeightsArgs), _P]),
+    "fcmoe_heaviest_positions": (_I, [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _P]),
+    "fcmoe_latent_cache_move": (_I, [ctypes.POINTER(LatentMoveArgs), _P]),
 }
 
 FCMOE_STAGE_COUNT = 24

@@ -1,0 +1,399 @@
+// fcmoe_latent_select.hip -- what lies between attentions over a part of a
+// latent cache: the masks of a tree of drafted tokens, the positions that a
+// sequence keeps, and the move of cached rows.
+#include "fcmoe_internal.h"
+#include "fcmoe_latent.h"
+
+namespace fcmoe {
+
+namespace {
+
+typedef __attribute__((address_space(3))) int32_t lds_i32;
+
+// ---- trees of drafted tokens --------------------------------------------------
+//
+// Node i of a sequence's n has parent[i] < i among them, or none. Its mask has
+// the bits of its line up to the root, its own included; its depth is the length
+// of that line but one. A workgroup a sequence: the parents go to LDS, and each
+// thread walks the line of one (node, mask word) pair until it lies before that
+// word: bound by the latency of a line's LDS reads.
+constexpr int kTreeNodes = 1024, kTreeThreads = 256;
+
+struct Tree {
+  const int32_t* parents;
+  const int32_t* starts;
+  int64_t tokens;
+  int batch, words;
+  uint64_t* masks;  // [tokens, words]
+  int32_t* depths;
+};
+
+__global__ __launch_bounds__(kTreeThreads) void draft_tree_kernel(const Tree p) {
+  __shared__ int parent[kTreeNodes];
+  __shared__ int tops[kTreeThreads / kWave];
+  const int b = (int)blockIdx.x, tid = (int)threadIdx.x;
+  // the sequence's span: a start below an earlier one counts as that one
+  int top = 0;
+  for (int k = tid; k <= b; k += kTreeThreads) top = max(top, (int)clamp64(p.starts[k], 0, p.tokens));
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) top = max(top, __shfl_xor(top, o));
+  if (tid % kWave == 0) tops[tid / kWave] = top;
+  __syncthreads();
+  for (int w = 0; w < kTreeThreads / kWave; ++w) top = max(top, tops[w]);
+  const int64_t q0 = top, end = max((int64_t)top, clamp64(p.starts[b + 1], 0, p.tokens));
+  // tokens before the first and behind the last sequence see nothing
+  auto clear = [&](int64_t from, int64_t to) {
+    for (int64_t k = from * p.words + tid; k < to * p.words; k += kTreeThreads) p.masks[k] = 0;
+    for (int64_t k = from + tid; k < to; k += kTreeThreads) p.depths[k] = 0;
+  };
+  if (b == 0) clear(0, q0);
+  if (b == p.batch - 1) clear(end, p.tokens);
+  const int64_t n = end - q0;
+  const int nodes = (int)(n < 64 * p.words ? n : 64 * p.words);  // nodes past them see the context alone
+  if (nodes < n) clear(q0 + nodes, end);
+  for (int i = tid; i < nodes; i += kTreeThreads) {
+    const int v = p.parents[q0 + i];
+    parent[i] = v >= 0 && v < i ? v : -1;
+  }
+  __syncthreads();
+  for (int k = tid; k < nodes * p.words; k += kTreeThreads) {
+    const int i = k / p.words, w = k - i * p.words;
+    uint64_t bits = 0;
+    int depth = -1;
+    for (int at = i; at >= (w == 0 ? 0 : 64 * w); at = parent[at]) {
+      if (at < 64 * w + 64) bits |= (uint64_t)1 << (at % 64);
+      ++depth;
+    }
+    p.masks[(q0 + i) * p.words + w] = bits;
+    if (w == 0) p.depths[q0 + i] = depth;
+  }
+}
+
+// ---- the positions that stay ----------------------------------------------------
+//
+// Of a sequence of len > keep tokens: its first `sinks`, its last `recent`, and of
+// the others the keep - sinks - recent with the largest weights, ties to the
+// lower position (NaN counts as the largest, -0 as 0), in ascending order.
+// A workgroup a sequence. The m-th largest weight is found from its bits, as
+// integers in the same order, 11, 11 and 10 at a time from the top: a histogram
+// in LDS of those that agree so far, then the bin that the m-th falls into. What
+// is kept is counted wave by wave and written in a second walk.
+constexpr int kHeavyWaves = 16, kBins = 2048, kCopies = 4;
+
+struct Heavy {
+  const float* weights;
+  int64_t positions, stride;
+  const int32_t* lens;
+  int64_t keep;
+  int sinks, recent;
+  int32_t* out;  // [batch, keep], -1 behind the count
+  int32_t* counts;
+  float* kept;   // [batch, keep], 0 behind the count
+};
+
+__device__ __forceinline__ uint32_t order_of(float w) {
+  if (w != w) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(w + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// Sum over the lanes before this one, and in *total over all.
+__device__ __forceinline__ int lanes_before(int v, int* total) {
+  int upto = v;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int u = __shfl_up(upto, o);
+    if ((int)threadIdx.x % kWave >= o) upto += u;
+  }
+  *total = __shfl(upto, kWave - 1);
+  return upto - v;
+}
+
+__global__ __launch_bounds__(kHeavyWaves* kWave) void heaviest_kernel(const Heavy p) {
+  constexpr int THREADS = kHeavyWaves * kWave;
+  __shared__ int hist[kCopies][kBins];
+  __shared__ int waves[2][kHeavyWaves];
+  __shared__ int found[2];  // digit, how many of its bin
+  const int64_t b = blockIdx.x;
+  const int tid = (int)threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const float* w = p.weights + b * p.stride;
+  int32_t* out = p.out + b * p.keep;
+  float* kept = p.kept + b * p.keep;
+  const int len = (int)clamp64(p.lens[b], 0, p.positions);
+  const int count = (int)(len < p.keep ? len : p.keep);
+  if (tid == 0) p.counts[b] = count;
+  for (int64_t k = count + tid; k < p.keep; k += THREADS) {
+    out[k] = -1;
+    kept[k] = 0.0f;
+  }
+  if (len <= p.keep) {
+    for (int k = tid; k < len; k += THREADS) {
+      out[k] = k;
+      kept[k] = w[k];
+    }
+    return;
+  }
+  const int first = p.sinks, last = len - p.recent;  // the others: [first, last)
+  for (int k = tid; k < p.sinks; k += THREADS) {
+    out[k] = k;
+    kept[k] = w[k];
+  }
+  for (int k = tid; k < p.recent; k += THREADS) {
+    out[p.keep - p.recent + k] = last + k;
+    kept[p.keep - p.recent + k] = w[last + k];
+  }
+  int need = (int)p.keep - p.sinks - p.recent;
+  if (need <= 0) return;
+
+  uint32_t prefix = 0, mask = 0;
+#pragma unroll
+  for (int round = 0; round < 3; ++round) {
+    const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
+    const uint32_t digits = round == 2 ? 1023u : 2047u;
+    for (int k = tid; k < kCopies * kBins; k += THREADS) hist[k / kBins][k % kBins] = 0;
+    __syncthreads();
+    for (int j = first + tid; j < last; j += THREADS) {
+      const uint32_t u = order_of(w[j]);
+      if ((u & mask) == prefix) atomicAdd(&hist[wave % kCopies][u >> shift & digits], 1);
+    }
+    __syncthreads();
+    // thread t has bins 2047 - 2 t and the one below: the largest first
+    const int hi = kBins - 1 - 2 * tid;
+    int n0 = 0, n1 = 0;
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+      n0 += hist[c][hi];
+      n1 += hist[c][hi - 1];
+    }
+    int total;
+    int before = lanes_before(n0 + n1, &total);
+    if (lane == 0) waves[0][wave] = total;
+    __syncthreads();
+    for (int v = 0; v < wave; ++v) before += waves[0][v];
+    if (before < need && before + n0 + n1 >= need) {
+      const bool upper = before + n0 >= need;
+      found[0] = upper ? hi : hi - 1;
+      found[1] = need - before - (upper ? 0 : n0);
+    }
+    __syncthreads();
+    prefix |= (uint32_t)found[0] << shift;
+    mask |= digits << shift;
+    need = found[1];
+  }
+  // what is above `prefix` stays, and the first `need` that equal it
+  const int blocks = (last - first + kWave - 1) / kWave;  // 64 positions each, in turn to the waves
+  const int k0 = (int)((int64_t)blocks * wave / kHeavyWaves), k1 = (int)((int64_t)blocks * (wave + 1) / kHeavyWaves);
+  int above = 0, same = 0;
+  for (int k = k0; k < k1; ++k) {
+    const int j = first + k * kWave + lane;
+    const uint32_t u = j < last ? order_of(w[j]) : 0;
+    above += __popcll(__ballot(j < last && u > prefix));
+    same += __popcll(__ballot(j < last && u == prefix));
+  }
+  if (lane == 0) {
+    waves[0][wave] = above;
+    waves[1][wave] = same;
+  }
+  __syncthreads();
+  int at = p.sinks, ties = 0;  // places taken before this wave's, ties among the positions before
+  for (int v = 0; v < wave; ++v) {
+    const int s = waves[1][v], stay = max(min(need - ties, s), 0);
+    at += waves[0][v] + stay;
+    ties += s;
+  }
+  const uint64_t lower = ((uint64_t)1 << lane) - 1;
+  for (int k = k0; k < k1; ++k) {
+    const int j = first + k * kWave + lane;
+    const float v = j < last ? w[j] : 0.0f;
+    const uint32_t u = order_of(v);
+    const uint64_t eq = __ballot(j < last && u == prefix);
+    const bool stays = j < last && (u > prefix || (u == prefix && ties + __popcll(eq & lower) < need));
+    const uint64_t all = __ballot(stays);
+    if (stays) {
+      const int to = at + __popcll(all & lower);
+      out[to] = j;
+      kept[to] = v;
+    }
+    at += __popcll(all);
+    ties += __popcll(eq);
+  }
+}
+
+// ---- moving cached rows ---------------------------------------------------------
+//
+// Row positions[b, k] of sequence b becomes its row starts[b] + k, for k < counts[b].
+// Bound by the rows' bytes, read once and written once.
+struct Move {
+  fcmoe_latent_cache c;
+  const int32_t* from;
+  int64_t from_width, from_stride;
+  const int32_t* to;
+  int64_t to_width, to_stride;
+  const int32_t* positions;  // [batch, most]
+  int64_t most, positions_stride;
+  const int32_t* counts;
+  const int32_t* starts;
+  int64_t batch;
+};
+
+__device__ __forceinline__ int move_count(const Move& p, int64_t b) { return (int)clamp64(p.counts[b], 0, p.most); }
+// The page and row of a position, or -1: none there.
+__device__ __forceinline__ int2 cached_at(const Move& p, const int32_t* table, int64_t width, int64_t at) {
+  const int64_t page = at / p.c.page_size;
+  if (at < 0 || page >= width) return make_int2(-1, 0);
+  const int32_t id = table[page];
+  if ((uint64_t)(int64_t)id >= (uint64_t)p.c.pages) return make_int2(-1, 0);
+  return make_int2(id, (int)(at - page * p.c.page_size));
+}
+
+// To rows that no row of the call is read from: every 16 bytes on their own.
+template <int R, int P, bool F8>
+__global__ __launch_bounds__(256) void move_apart_kernel(const Move p) {
+  constexpr int ELEM = F8 ? 1 : 2, LU = R * ELEM / 16, UNITS = LU + P * ELEM / 16, ROWS = 16;
+  __shared__ int2 src[ROWS], dst[ROWS];
+  const int64_t b = blockIdx.y;
+  const int count = move_count(p, b), k0 = (int)blockIdx.x * ROWS, tid = (int)threadIdx.x;
+  if (k0 >= count) return;
+  if (tid < ROWS) {
+    const int k = k0 + tid;
+    int2 s = make_int2(-1, 0), d = make_int2(-1, 0);
+    if (k < count) {
+      s = cached_at(p, p.from + b * p.from_stride, p.from_width, p.positions[b * p.positions_stride + k]);
+      d = cached_at(p, p.to + b * p.to_stride, p.to_width, (p.starts ? (int64_t)p.starts[b] : 0) + k);
+    }
+    if (d.x < 0) s.x = -1;
+    src[tid] = s, dst[tid] = d;
+    if (F8 && s.x >= 0) p.c.scale[d.x * p.c.scale_page_stride + d.y] = p.c.scale[s.x * p.c.scale_page_stride + s.y];
+  }
+  __syncthreads();
+  constexpr int EACH = (ROWS * UNITS + 255) / 256;
+  v4i v[EACH];
+  auto place = [&](int2 at, int unit) {
+    return unit < LU ? (char*)p.c.latent + (at.x * p.c.latent_page_stride + at.y * p.c.latent_row_stride) * ELEM + unit * 16
+                     : (char*)p.c.rope + (at.x * p.c.rope_page_stride + at.y * p.c.rope_row_stride) * ELEM + (unit - LU) * 16;
+  };
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int at = i * 256 + tid, row = at / UNITS;
+    if (row < ROWS && src[row].x >= 0) v[i] = *(const v4i*)place(src[row], at % UNITS);
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int at = i * 256 + tid, row = at / UNITS;
+    if (row < ROWS && src[row].x >= 0) *(v4i*)place(dst[row], at % UNITS) = v[i];
+  }
+}
+
+// Within a sequence: positions ascend and none lies before its new place, so a
+// row's place is only ever read for an earlier one (or itself). A workgroup takes
+// 128 bytes of every row of a sequence (the last one the key part and the
+// scales), 1024 rows at a time in order: they are all read before any is written.
+template <int R, int P, bool F8>
+__global__ __launch_bounds__(1024) void move_within_kernel(const Move p) {
+  constexpr int ELEM = F8 ? 1 : 2, PIECES = R * ELEM / 128, RU = P * ELEM / 16, HOLD = 8;
+  const int64_t b = blockIdx.y;
+  const int count = move_count(p, b), piece = (int)blockIdx.x, unit = (int)threadIdx.x % 8;
+  const int64_t first = p.starts ? p.starts[b] : 0;
+  const bool latent = piece < PIECES, rope = !latent && unit < RU, scale = F8 && !latent && unit == 7;
+  for (int k0 = 0; k0 < count; k0 += 128 * HOLD) {
+    v4i v[HOLD];
+    int2 to[HOLD];
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i) {
+      const int k = k0 + i * 128 + (int)threadIdx.x / 8;
+      to[i] = make_int2(-1, 0);
+      if (k >= count) continue;
+      const int64_t at = p.positions[b * p.positions_stride + k];
+      if (at == first + k) continue;
+      const int2 s = cached_at(p, p.from + b * p.from_stride, p.from_width, at);
+      if (s.x >= 0) to[i] = cached_at(p, p.from + b * p.from_stride, p.from_width, first + k);
+      if (to[i].x < 0) continue;
+      if (latent)
+        v[i] = *(const v4i*)((const char*)p.c.latent + (s.x * p.c.latent_page_stride + s.y * p.c.latent_row_stride) * ELEM + piece * 128 + unit * 16);
+      else if (rope)
+        v[i] = *(const v4i*)((const char*)p.c.rope + (s.x * p.c.rope_page_stride + s.y * p.c.rope_row_stride) * ELEM + unit * 16);
+      else if (scale)
+        v[i][0] = __float_as_int(p.c.scale[s.x * p.c.scale_page_stride + s.y]);
+    }
+    loads_barrier();  // all of them are here before the first is overwritten
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i) {
+      if (to[i].x < 0) continue;
+      if (latent)
+        *(v4i*)((char*)p.c.latent + (to[i].x * p.c.latent_page_stride + to[i].y * p.c.latent_row_stride) * ELEM + piece * 128 + unit * 16) = v[i];
+      else if (rope)
+        *(v4i*)((char*)p.c.rope + (to[i].x * p.c.rope_page_stride + to[i].y * p.c.rope_row_stride) * ELEM + unit * 16) = v[i];
+      else if (scale)
+        p.c.scale[to[i].x * p.c.scale_page_stride + to[i].y] = __int_as_float(v[i][0]);
+    }
+  }
+}
+
+template <int R, int P, bool F8>
+void move_launch(const Move& p, hipStream_t stream) {
+  if (p.to)
+    hipLaunchKernelGGL((move_apart_kernel<R, P, F8>), dim3((unsigned)ceil_div(p.most, 16), (unsigned)p.batch), dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL((move_within_kernel<R, P, F8>), dim3((unsigned)(R * (F8 ? 1 : 2) / 128 + (P || F8 ? 1 : 0)), (unsigned)p.batch),
+                       dim3(1024), 0, stream, p);
+}
+
+}  // namespace
+
+}  // namespace fcmoe
+
+using namespace fcmoe;
+
+extern "C" int fcmoe_draft_tree(const int32_t* parents, int64_t tokens, const int32_t* query_starts, int64_t batch,
+                                int64_t mask_words, uint64_t* masks, int32_t* depths, hipStream_t stream) {
+  if (tokens < 0 || tokens > INT32_MAX || batch <= 0 || batch > (1 << 20) || mask_words < 1 || mask_words > kTreeNodes / 64)
+    return fail(FCMOE_EINVAL, "draft_tree: bad shape (1 to 16 mask words)");
+  if (tokens == 0) return FCMOE_OK;
+  if (!parents || !query_starts || !masks || !depths) return fail(FCMOE_EINVAL, "draft_tree: NULL pointer");
+  Tree p{parents, query_starts, tokens, (int)batch, (int)mask_words, masks, depths};
+  hipLaunchKernelGGL(draft_tree_kernel, dim3((unsigned)batch), dim3(kTreeThreads), 0, stream, p);
+  return check_launch("draft_tree");
+}
+
+extern "C" int fcmoe_heaviest_positions(const float* weights, int64_t batch, int64_t positions, int64_t stride,
+                                        const int32_t* kv_lens, int64_t keep, int64_t sinks, int64_t recent,
+                                        int32_t* out_positions, int32_t* counts, float* kept, hipStream_t stream) {
+  if (batch < 0 || batch > (1 << 20) || positions < 0 || positions > INT32_MAX - 4096 || stride < 0 || keep < 1 || keep > INT32_MAX - 4096 ||
+      sinks < 0 || recent < 0 || sinks > keep || recent > keep - sinks)
+    return fail(FCMOE_EINVAL, "heaviest_positions: bad shape (keep at least 1, and no fewer than sinks + recent)");
+  if (batch == 0) return FCMOE_OK;
+  if ((positions > 0 && !weights) || !kv_lens || !out_positions || !counts || !kept)
+    return fail(FCMOE_EINVAL, "heaviest_positions: NULL pointer");
+  Heavy p{weights, positions, stride, kv_lens, keep, (int)sinks, (int)recent, out_positions, counts, kept};
+  hipLaunchKernelGGL(heaviest_kernel, dim3((unsigned)batch), dim3(kHeavyWaves * kWave), 0, stream, p);
+  return check_launch("heaviest_positions");
+}
+
+extern "C" int fcmoe_latent_cache_move(const fcmoe_latent_move_args* a, hipStream_t stream) {
+  if (!a) return fail(FCMOE_EINVAL, "latent_cache_move: NULL args");
+  if (const int rc = check_latent_cache(a->cache, "latent_cache_move")) return rc;
+  if (a->batch < 0 || a->batch > 65535 || a->most < 0 || a->most > INT32_MAX - 4096 || a->positions_stride < 0 || a->table_width < 0 ||
+      a->table_width > INT32_MAX || a->page_table_stride < 0 || a->to_width < 0 || a->to_width > INT32_MAX || a->to_stride < 0)
+    return fail(FCMOE_EINVAL, "latent_cache_move: bad shape");
+  if (a->batch == 0 || a->most == 0 || a->cache.pages == 0 || a->table_width == 0) return FCMOE_OK;
+  if (!a->page_table || !a->positions || !a->counts) return fail(FCMOE_EINVAL, "latent_cache_move: NULL pointer");
+  Move p{};
+  p.c = a->cache;
+  p.from = a->page_table, p.from_width = a->table_width, p.from_stride = a->page_table_stride;
+  p.to = a->to_table, p.to_width = a->to_width, p.to_stride = a->to_stride;
+  p.positions = a->positions, p.most = a->most, p.positions_stride = a->positions_stride;
+  p.counts = a->counts, p.starts = a->starts, p.batch = a->batch;
+  const bool f8 = a->cache.e4m3 != 0;
+  if (a->cache.latent_dim == 512) {
+    if (a->cache.rope_dim == 64)
+      f8 ? move_launch<512, 64, true>(p, stream) : move_launch<512, 64, false>(p, stream);
+    else
+      f8 ? move_launch<512, 0, true>(p, stream) : move_launch<512, 0, false>(p, stream);
+  } else {
+    if (a->cache.rope_dim == 64)
+      f8 ? move_launch<256, 64, true>(p, stream) : move_launch<256, 64, false>(p, stream);
+    else
+      f8 ? move_launch<256, 0, true>(p, stream) : move_launch<256, 0, false>(p, stream);
+  }
+  return check_launch("latent_cache_move");
+}

@@ -468,12 +468,25 @@ void check_starts(const at::Tensor& t, int64_t batch, const char* name) {
   TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == batch + 1, name, " must be [", batch + 1, "], got ", t.sizes());
 }
 
+// A window and the first tokens beside it: sinks without a window would change nothing.
+fcmoe_key_mask check_window(c10::optional<int64_t> window, int64_t sinks, const char* what) {
+  fcmoe_key_mask m{};
+  TORCH_CHECK_VALUE(!window.has_value() || *window >= 1, what, ": window must be at least 1, got ", *window);
+  TORCH_CHECK_VALUE(sinks >= 0, what, ": sinks must not be negative, got ", sinks);
+  TORCH_CHECK_VALUE(window.has_value() || sinks == 0, what, ": sinks need a window");
+  m.window = window.value_or(0), m.sinks = sinks;
+  return m;
+}
+
 std::tuple<at::Tensor, OptTensor> absorbed_attention(at::Tensor q_latent, OptTensor q_rope_, at::Tensor latent,
                                                      OptTensor rope_, OptTensor scale_, at::Tensor page_table,
                                                      at::Tensor kv_lens, OptTensor query_starts, double scale,
-                                                     OptTensor out, bool return_lse) {
+                                                     OptTensor out, bool return_lse, c10::optional<int64_t> window,
+                                                     int64_t sinks, OptTensor masks_, OptTensor depths_) {
   const char* what = "absorbed_attention";
   const at::Tensor q_rope = opt(q_rope_), rope = opt(rope_), cache_scale = opt(scale_), starts = opt(query_starts);
+  const at::Tensor masks = opt(masks_), depths = opt(depths_);
+  fcmoe_key_mask km = check_window(window, sinks, what);
   fcmoe_absorbed_args a{};
   a.cache = check_cache(latent, rope, cache_scale, what);
   check_dtype(q_latent, at::kBFloat16, "q_latent");
@@ -497,15 +510,25 @@ std::tuple<at::Tensor, OptTensor> absorbed_attention(at::Tensor q_latent, OptTen
   } else {
     TORCH_CHECK_VALUE(T == B, "without query_starts there is one query token a sequence: got ", T, " and ", B);
   }
+  if (masks.defined()) {
+    TORCH_CHECK_VALUE(starts.defined(), "a tree needs query_starts");
+    check_dtype(masks, at::kLong, "tree.masks");
+    TORCH_CHECK_VALUE(masks.dim() == 2 && masks.size(0) == T && masks.size(1) >= 1 && masks.size(1) <= 16,
+                      "tree.masks must be [", T, ", 1 to 16 words], got ", masks.sizes());
+    TORCH_CHECK_VALUE(T * masks.size(1) < (1 << 27), "tree.masks must be below 1 GiB, got ", masks.sizes());
+    TORCH_CHECK_VALUE(depths.defined(), "a tree has masks and depths");
+    check_dtype(depths, at::kInt, "tree.depths");
+    TORCH_CHECK_VALUE(depths.dim() == 1 && depths.size(0) == T, "tree.depths must be [", T, "], got ", depths.sizes());
+  }
   TORCH_CHECK_VALUE(B <= (1 << 20) && T * H <= INT32_MAX / 2, "too many sequences or query rows");
   check_scale(scale, what);
   check_output(out, {T, H, R}, what);
   const at::Tensor given = opt(out);
   check_no_grad({&q_latent, &q_rope, &latent, &rope, &cache_scale}, what);
   if (given.defined())
-    check_written({{&given, "out"}}, {&q_latent, &q_rope, &latent, &rope, &cache_scale, &page_table, &kv_lens, &starts},
+    check_written({{&given, "out"}}, {&q_latent, &q_rope, &latent, &rope, &cache_scale, &page_table, &kv_lens, &starts, &masks, &depths},
                   what);
-  check_devices(q_latent, {&q_rope, &latent, &rope, &cache_scale, &page_table, &kv_lens, &starts, &given}, what);
+  check_devices(q_latent, {&q_rope, &latent, &rope, &cache_scale, &page_table, &kv_lens, &starts, &given, &masks, &depths}, what);
   c10::DeviceGuard guard(q_latent.device());
   Out o = output(out, {T, H, R}, q_latent, 4, what);
   OptTensor lse;
@@ -528,12 +551,19 @@ std::tuple<at::Tensor, OptTensor> absorbed_attention(at::Tensor q_latent, OptTen
   a.out_token_stride = stride_at(o.direct, 0), a.out_head_stride = stride_at(o.direct, 1);
   a.lse = return_lse ? lse->data_ptr<float>() : nullptr;
   a.zero_uncovered = !o.given;
-  a.workspace_bytes = fcmoe_absorbed_attention_workspace_bytes(&a);
+  const bool masked = window.has_value() || masks.defined();
+  const at::Tensor words = masks.defined() ? masks.contiguous() : masks, depth = depths.defined() ? depths.contiguous() : depths;
+  if (masks.defined()) {
+    km.tree_masks = (const uint64_t*)words.data_ptr<int64_t>(), km.mask_words = km.mask_stride = words.size(1);
+    km.tree_depths = depth.data_ptr<int32_t>();
+  }
+  a.workspace_bytes = masked ? fcmoe_absorbed_attention_masked_workspace_bytes(&a, &km) : fcmoe_absorbed_attention_workspace_bytes(&a);
   at::Tensor ws = at::empty({(int64_t)a.workspace_bytes}, q_latent.options().dtype(at::kByte));
   a.workspace = ws.data_ptr();
   {
     pybind11::gil_scoped_release release;
-    check_rc(fcmoe_absorbed_attention(&a, stream_of(q_latent)), what);
+    check_rc(masked ? fcmoe_absorbed_attention_masked(&a, &km, stream_of(q_latent)) : fcmoe_absorbed_attention(&a, stream_of(q_latent)),
+             what);
   }
   finish(o);
   return {o.result, lse};
@@ -541,8 +571,11 @@ std::tuple<at::Tensor, OptTensor> absorbed_attention(at::Tensor q_latent, OptTen
 
 std::tuple<at::Tensor, OptTensor> expanded_attention(at::Tensor q, at::Tensor kv, OptTensor k_rope_,
                                                      at::Tensor query_starts, OptTensor kv_starts_, double scale,
-                                                     bool causal, OptTensor out, bool return_lse) {
+                                                     bool causal, OptTensor out, bool return_lse,
+                                                     c10::optional<int64_t> window, int64_t sinks) {
   const char* what = "expanded_attention";
+  const fcmoe_key_mask km = check_window(window, sinks, what);
+  TORCH_CHECK_VALUE(causal || !window.has_value(), what, ": a window needs causal=True");
   const at::Tensor k_rope = opt(k_rope_);
   const at::Tensor kv_starts = has(kv_starts_) ? *kv_starts_ : query_starts;
   check_dtype(q, at::kBFloat16, "q");
@@ -601,7 +634,8 @@ std::tuple<at::Tensor, OptTensor> expanded_attention(at::Tensor q, at::Tensor kv
   a.out_token_stride = stride_at(o.direct, 0), a.out_head_stride = stride_at(o.direct, 1);
   a.lse = return_lse ? lse->data_ptr<float>() : nullptr;
   a.zero_uncovered = !o.given;
-  a.workspace_bytes = fcmoe_expanded_attention_workspace_bytes(&a);
+  const bool masked = window.has_value();
+  a.workspace_bytes = masked ? fcmoe_expanded_attention_masked_workspace_bytes(&a, &km) : fcmoe_expanded_attention_workspace_bytes(&a);
   at::Tensor ws;
   if (a.workspace_bytes) {
     ws = at::empty({(int64_t)a.workspace_bytes}, q.options().dtype(at::kByte));
@@ -609,10 +643,200 @@ std::tuple<at::Tensor, OptTensor> expanded_attention(at::Tensor q, at::Tensor kv
   }
   {
     pybind11::gil_scoped_release release;
-    check_rc(fcmoe_expanded_attention(&a, stream_of(q)), what);
+    check_rc(masked ? fcmoe_expanded_attention_masked(&a, &km, stream_of(q)) : fcmoe_expanded_attention(&a, stream_of(q)), what);
   }
   finish(o);
   return {o.result, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor> draft_tree(at::Tensor parents, at::Tensor query_starts, int64_t max_nodes) {
+  const char* what = "draft_tree";
+  check_dtype(parents, at::kInt, "parents");
+  check_dim(parents, 1, "parents", "[tokens]");
+  check_dtype(query_starts, at::kInt, "query_starts");
+  TORCH_CHECK_VALUE(query_starts.dim() == 1 && query_starts.size(0) >= 1, "query_starts must be [sequences + 1], got ",
+                    query_starts.sizes());
+  TORCH_CHECK_VALUE(max_nodes >= 1 && max_nodes <= 1024, "max_nodes must be 1 to 1024, got ", max_nodes);
+  const int64_t T = parents.size(0), B = query_starts.size(0) - 1, words = (max_nodes + 63) / 64;
+  TORCH_CHECK_VALUE(B <= (1 << 20) && T <= INT32_MAX, "too many sequences or tokens");
+  check_devices(parents, {&query_starts}, what);
+  c10::DeviceGuard guard(parents.device());
+  at::Tensor masks = at::empty({T, words}, parents.options().dtype(at::kLong)), depths = at::empty({T}, parents.options());
+  if (T == 0) return {masks, depths};
+  if (B == 0) return {masks.zero_(), depths.zero_()};
+  const at::Tensor ps = parents.contiguous(), st = query_starts.contiguous();
+  {
+    pybind11::gil_scoped_release release;
+    check_rc(fcmoe_draft_tree(ps.data_ptr<int32_t>(), T, st.data_ptr<int32_t>(), B, words, (uint64_t*)masks.data_ptr<int64_t>(),
+                              depths.data_ptr<int32_t>(), stream_of(parents)),
+             what);
+  }
+  return {masks, depths};
+}
+
+// Rows [sequences, positions] of fp32 whose values lie side by side.
+bool weight_rows_ok(const at::Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1; }
+
+at::Tensor attention_weights(at::Tensor q_latent, OptTensor q_rope_, at::Tensor latent, OptTensor rope_, OptTensor scale_,
+                             at::Tensor page_table, at::Tensor kv_lens, at::Tensor lse, double scale, OptTensor query_starts,
+                             OptTensor previous_, OptTensor out) {
+  const char* what = "attention_weights";
+  const at::Tensor q_rope = opt(q_rope_), rope = opt(rope_), cache_scale = opt(scale_), starts = opt(query_starts);
+  const at::Tensor previous = opt(previous_), given = opt(out);
+  fcmoe_attention_weights_args a{};
+  a.cache = check_cache(latent, rope, cache_scale, what);
+  check_dtype(q_latent, at::kBFloat16, "q_latent");
+  TORCH_CHECK_VALUE(q_latent.dim() == 3 && q_latent.size(1) > 0 && q_latent.size(1) <= 65536 &&
+                        q_latent.size(2) == a.cache.latent_dim,
+                    "q_latent must be [tokens, heads, ", a.cache.latent_dim, "], got ", q_latent.sizes());
+  const int64_t T = q_latent.size(0), H = q_latent.size(1);
+  TORCH_CHECK_VALUE(q_rope.defined() == rope.defined(), "q_rope goes with a cache that has a rope part");
+  if (q_rope.defined()) {
+    check_dtype(q_rope, at::kBFloat16, "q_rope");
+    TORCH_CHECK_VALUE(q_rope.dim() == 3 && q_rope.size(0) == T && q_rope.size(1) == H && q_rope.size(2) == a.cache.rope_dim,
+                      "q_rope must be [", T, ", ", H, ", ", a.cache.rope_dim, "], got ", q_rope.sizes());
+  }
+  check_dtype(page_table, at::kInt, "page_table");
+  check_dim(page_table, 2, "page_table", "[sequences, pages]");
+  const int64_t B = page_table.size(0);
+  check_dtype(kv_lens, at::kInt, "kv_lens");
+  TORCH_CHECK_VALUE(kv_lens.dim() == 1 && kv_lens.size(0) == B, "kv_lens must be [", B, "], got ", kv_lens.sizes());
+  if (starts.defined()) {
+    check_starts(starts, B, "query_starts");
+  } else {
+    TORCH_CHECK_VALUE(T == B, "without query_starts there is one query token a sequence: got ", T, " and ", B);
+  }
+  check_dtype(lse, at::kFloat, "lse");
+  TORCH_CHECK_VALUE(lse.dim() == 2 && lse.size(0) == T && lse.size(1) == H, "lse must be [", T, ", ", H, "], got ", lse.sizes());
+  TORCH_CHECK_VALUE(B <= 65535 && T * H <= INT32_MAX / 2, "too many sequences or query rows");
+  int64_t S = page_table.size(1) * a.cache.page_size;
+  if (previous.defined()) {
+    check_dtype(previous, at::kFloat, "previous");
+    TORCH_CHECK_VALUE(previous.dim() == 2 && previous.size(0) == B, "previous must be [", B, ", positions], got ", previous.sizes());
+    S = previous.size(1);
+  }
+  if (given.defined()) {
+    check_dtype(given, at::kFloat, "out");
+    if (!previous.defined() && given.dim() == 2) S = given.size(1);
+    TORCH_CHECK_VALUE(given.dim() == 2 && given.size(0) == B && given.size(1) == S, "out must be [", B, ", ", S, "], got ", given.sizes());
+    TORCH_CHECK_VALUE(weight_rows_ok(given), "out must have contiguous rows");
+    TORCH_CHECK(!given.requires_grad() && !has_tangent(given), what, ": out with requires_grad=True is not supported, nor one with a tangent");
+  }
+  TORCH_CHECK_VALUE(S <= INT32_MAX - 512, "too many positions");
+  check_scale(scale, what);
+  check_no_grad({&q_latent, &q_rope, &latent, &rope, &cache_scale, &lse, &previous}, what);
+  const bool in_place = given.defined() && previous.defined() && given.data_ptr() == previous.data_ptr() &&
+                        stride_at(given, 0) == stride_at(previous, 0) && stride_at(given, 1) == stride_at(previous, 1);
+  const at::Tensor none;
+  if (given.defined())
+    check_written({{&given, "out (unless it is previous itself)"}},
+                  {&q_latent, &q_rope, &latent, &rope, &cache_scale, &page_table, &kv_lens, &starts, &lse, in_place ? &none : &previous}, what);
+  check_devices(q_latent, {&q_rope, &latent, &rope, &cache_scale, &page_table, &kv_lens, &starts, &lse, &previous, &given}, what);
+  c10::DeviceGuard guard(q_latent.device());
+  const at::Tensor result = given.defined() ? given : at::empty({B, S}, q_latent.options().dtype(at::kFloat));
+  if (B == 0 || S == 0) return result;
+  cache_pointers(a.cache, latent, rope, cache_scale);
+  const at::Tensor ql = rows_for(q_latent, 8), qr = q_rope.defined() ? rows_for(q_rope, 8) : q_rope;
+  const at::Tensor table = page_table.size(1) > 1 && page_table.stride(1) != 1 ? page_table.contiguous() : page_table;
+  const at::Tensor lens = kv_lens.contiguous(), st = starts.defined() ? starts.contiguous() : starts, sums = lse.contiguous();
+  const at::Tensor before = previous.defined() && !weight_rows_ok(previous) ? previous.contiguous() : previous;
+  a.q_latent = bf16(ql), a.q_rope = bf16(qr);
+  a.tokens = T, a.heads = H, a.batch = B;
+  a.q_latent_token_stride = stride_at(ql, 0), a.q_latent_head_stride = stride_at(ql, 1);
+  if (qr.defined()) a.q_rope_token_stride = stride_at(qr, 0), a.q_rope_head_stride = stride_at(qr, 1);
+  a.page_table = table.data_ptr<int32_t>(), a.table_width = table.size(1), a.page_table_stride = stride_at(table, 0);
+  a.kv_lens = lens.data_ptr<int32_t>(), a.query_starts = st.defined() ? st.data_ptr<int32_t>() : nullptr;
+  a.lse = sums.data_ptr<float>(), a.scale = (float)scale;
+  a.previous = before.defined() ? before.data_ptr<float>() : nullptr;
+  a.previous_stride = before.defined() ? stride_at(before, 0) : 0;
+  a.out = result.data_ptr<float>(), a.out_stride = stride_at(result, 0), a.positions = S;
+  a.workspace_bytes = fcmoe_attention_weights_workspace_bytes(&a);
+  at::Tensor ws;
+  if (a.workspace_bytes) {
+    ws = at::empty({(int64_t)a.workspace_bytes}, q_latent.options().dtype(at::kByte));
+    a.workspace = ws.data_ptr();
+  }
+  {
+    pybind11::gil_scoped_release release;
+    check_rc(fcmoe_attention_weights(&a, stream_of(q_latent)), what);
+  }
+  if (given.defined()) was_written(given);
+  return result;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> heaviest_positions(at::Tensor weights, at::Tensor kv_lens, int64_t keep, int64_t sinks,
+                                                                  int64_t recent) {
+  const char* what = "heaviest_positions";
+  check_dtype(weights, at::kFloat, "weights");
+  check_dim(weights, 2, "weights", "[sequences, positions]");
+  const int64_t B = weights.size(0), S = weights.size(1);
+  check_dtype(kv_lens, at::kInt, "kv_lens");
+  TORCH_CHECK_VALUE(kv_lens.dim() == 1 && kv_lens.size(0) == B, "kv_lens must be [", B, "], got ", kv_lens.sizes());
+  TORCH_CHECK_VALUE(keep >= 1 && keep <= INT32_MAX - 4096, "keep must be at least 1, got ", keep);
+  TORCH_CHECK_VALUE(sinks >= 0 && recent >= 0 && sinks <= keep && recent <= keep - sinks,
+                    "sinks and recent must not be negative, nor more than keep together: got ", sinks, ", ", recent, " of ", keep);
+  TORCH_CHECK_VALUE(B <= (1 << 20) && S <= INT32_MAX - 4096, "too many sequences or positions");
+  check_no_grad({&weights}, what);
+  check_devices(weights, {&kv_lens}, what);
+  c10::DeviceGuard guard(weights.device());
+  const at::TensorOptions ints = weights.options().dtype(at::kInt);
+  at::Tensor positions = at::empty({B, keep}, ints), counts = at::empty({B}, ints), kept = at::empty({B, keep}, weights.options());
+  if (B == 0) return {positions, counts, kept};
+  const at::Tensor w = weight_rows_ok(weights) ? weights : weights.contiguous(), lens = kv_lens.contiguous();
+  {
+    pybind11::gil_scoped_release release;
+    check_rc(fcmoe_heaviest_positions(w.data_ptr<float>(), B, S, stride_at(w, 0), lens.data_ptr<int32_t>(), keep, sinks, recent,
+                                      positions.data_ptr<int32_t>(), counts.data_ptr<int32_t>(), kept.data_ptr<float>(), stream_of(weights)),
+             what);
+  }
+  return {positions, counts, kept};
+}
+
+void latent_cache_move(at::Tensor latent, OptTensor rope_, OptTensor scale_, at::Tensor page_table, at::Tensor positions, at::Tensor counts,
+                       OptTensor starts_, OptTensor to_table_) {
+  const char* what = "latent_cache_move";
+  const at::Tensor rope = opt(rope_), scale = opt(scale_), starts = opt(starts_), to_table = opt(to_table_);
+  fcmoe_latent_move_args a{};
+  a.cache = check_cache(latent, rope, scale, what);
+  check_dtype(page_table, at::kInt, "page_table");
+  check_dim(page_table, 2, "page_table", "[sequences, pages]");
+  const int64_t B = page_table.size(0);
+  check_dtype(positions, at::kInt, "positions");
+  TORCH_CHECK_VALUE(positions.dim() == 2 && positions.size(0) == B, "positions must be [", B, ", rows], got ", positions.sizes());
+  check_dtype(counts, at::kInt, "counts");
+  TORCH_CHECK_VALUE(counts.dim() == 1 && counts.size(0) == B, "counts must be [", B, "], got ", counts.sizes());
+  if (starts.defined()) {
+    check_dtype(starts, at::kInt, "starts");
+    TORCH_CHECK_VALUE(starts.dim() == 1 && starts.size(0) == B, "starts must be [", B, "], got ", starts.sizes());
+  }
+  if (to_table.defined()) {
+    check_dtype(to_table, at::kInt, "to_table");
+    TORCH_CHECK_VALUE(to_table.dim() == 2 && to_table.size(0) == B, "to_table must be [", B, ", pages], got ", to_table.sizes());
+  }
+  TORCH_CHECK_VALUE(B <= 65535 && positions.size(1) <= INT32_MAX - 4096, "too many sequences or rows");
+  check_no_grad({&latent, &rope, &scale}, what);
+  check_written({{&latent, "cache.latent"}, {&rope, "cache.rope"}, {&scale, "cache.scale"}}, {&page_table, &positions, &counts, &starts, &to_table},
+                what);
+  check_devices(latent, {&rope, &scale, &page_table, &positions, &counts, &starts, &to_table}, what);
+  c10::DeviceGuard guard(latent.device());
+  if (B == 0 || positions.size(1) == 0) return;
+  cache_pointers(a.cache, latent, rope, scale);
+  auto rows = [](const at::Tensor& t) { return t.size(1) > 1 && t.stride(1) != 1 ? t.contiguous() : t; };
+  const at::Tensor from = rows(page_table), to = to_table.defined() ? rows(to_table) : to_table, at_ = rows(positions);
+  const at::Tensor n = counts.contiguous(), st = starts.defined() ? starts.contiguous() : starts;
+  // a table without pages has rows to move to nowhere
+  if (from.size(1) == 0 || (to.defined() && to.size(1) == 0)) return;
+  a.page_table = from.data_ptr<int32_t>(), a.table_width = from.size(1), a.page_table_stride = stride_at(from, 0);
+  if (to.defined()) a.to_table = to.data_ptr<int32_t>(), a.to_width = to.size(1), a.to_stride = stride_at(to, 0);
+  a.positions = at_.data_ptr<int32_t>(), a.most = at_.size(1), a.positions_stride = stride_at(at_, 0);
+  a.counts = n.data_ptr<int32_t>(), a.starts = st.defined() ? st.data_ptr<int32_t>() : nullptr, a.batch = B;
+  {
+    pybind11::gil_scoped_release release;
+    check_rc(fcmoe_latent_cache_move(&a, stream_of(latent)), what);
+  }
+  was_written(latent);
+  was_written(rope);
+  was_written(scale);
 }
 
 }  // namespace
@@ -624,4 +848,8 @@ void bind_latent_attention(pybind11::module_& m) {
   m.def("latent_head_projection", &head_projection);
   m.def("latent_absorbed_attention", &absorbed_attention);
   m.def("latent_expanded_attention", &expanded_attention);
+  m.def("latent_draft_tree", &draft_tree);
+  m.def("latent_attention_weights", &attention_weights);
+  m.def("latent_heaviest_positions", &heaviest_positions);
+  m.def("latent_cache_move", &latent_cache_move);
 }

@@ -20,6 +20,10 @@ values, ``rope_dim`` rotated key values beside them) lies in a paged cache:
     rows = latent_cache_append(..., return_rows=True)
     values = expanded_attention(q, kv_up, rows[:, latent_dim:], query_starts, scale=...)
 
+Both attentions take a sliding ``window`` with the first tokens that stay visible
+beside it (``sinks``); trees of drafted tokens and a cache that keeps its heavy
+tokens are in ``fused_cpp_amd.latent_context``.
+
 Everything is bf16 in and out. Norms, rotations, scores, softmax sums and all
 accumulators are fp32; the attentions round each softmax weight once to bf16 for
 its product with the values (times its token's scale in an e4m3 cache). The cache
@@ -74,6 +78,15 @@ def allocate_latent_cache(pages: int, page_size: int, *, latent_dim: int = 512, 
 
     return LatentCache(zeros(latent_dim), zeros(rope_dim) if rope_dim else None,
                        torch.zeros((pages, page_size), device=device) if dtype != torch.bfloat16 else None)
+
+
+@dataclass(frozen=True)
+class DraftTree:
+    """What the nodes of drafted trees see of one another: ``masks [tokens, words]`` int64, bit ``j % 64`` of word
+    ``j // 64`` for node j of the same sequence, and ``depths [tokens]`` int32, the roots' 0."""
+
+    masks: torch.Tensor
+    depths: torch.Tensor
 
 
 @dataclass(frozen=True)
@@ -134,7 +147,8 @@ def head_projection(x: torch.Tensor, weight: PreparedHeadProjection, *, out: Opt
 
 def absorbed_attention(q_latent: torch.Tensor, q_rope: Optional[torch.Tensor], cache: LatentCache,
                        page_table: torch.Tensor, kv_lens: torch.Tensor, *, scale: float,
-                       query_starts: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                       query_starts: Optional[torch.Tensor] = None, window: Optional[int] = None, sinks: int = 0,
+                       tree: Optional[DraftTree] = None, out: Optional[torch.Tensor] = None,
                        return_lse: bool = False):
     """Attention of queries in the latent space over the paged cache: ``[T, H, latent_dim]``.
 
@@ -146,29 +160,41 @@ def absorbed_attention(q_latent: torch.Tensor, q_rope: Optional[torch.Tensor], c
     cut to it, a page id outside the cache makes its sequence NaN. Cached tokens that a sequence's queries do not all
     see have to be finite; rows past a length may hold anything.
 
+    ``window``: a query sees its last ``window`` tokens, its own included, and the sequence's first ``sinks``. Only
+    pages that hold a token which some query sees are read, so the others may be gone (their table entries anything).
+    ``tree`` (of :func:`~fused_cpp_amd.latent_context.draft_tree`, with ``query_starts``): a sequence's n query tokens
+    are the nodes of a tree of drafts, cached in their order as its last n tokens. A node sees the ``kv_lens[b] - n`` tokens before them and the nodes that its mask has;
+    with a window the ones before them as a token at ``kv_lens[b] - n + depth`` does, and of the nodes still all that
+    its mask has. Nodes past the masks' words are not seen. Rows of nodes that a sequence's others see have to be
+    finite.
+
     ``return_lse`` adds ``[T, H]`` fp32: the log of the softmax's sum (-inf where there is none), which joins results
     over parts of a context. Tokens that no sequence holds are 0, or left as they were in a given ``out``.
     """
+    if tree is not None and not isinstance(tree, DraftTree):
+        raise TypeError("tree must come from latent_context.draft_tree")
     o, lse = _native.require_native().latent_absorbed_attention(
         q_latent, q_rope, cache.latent, cache.rope, cache.scale, page_table, kv_lens, query_starts, scale, out,
-        return_lse)
+        return_lse, window, sinks, None if tree is None else tree.masks, None if tree is None else tree.depths)
     return (o, lse) if return_lse else o
 
 
 def expanded_attention(q: torch.Tensor, kv: torch.Tensor, k_rope: Optional[torch.Tensor], query_starts: torch.Tensor,
                        *, scale: float, kv_starts: Optional[torch.Tensor] = None, causal: bool = True,
-                       out: Optional[torch.Tensor] = None, return_lse: bool = False):
+                       window: Optional[int] = None, sinks: int = 0, out: Optional[torch.Tensor] = None,
+                       return_lse: bool = False):
     """Attention over per-head keys and values ``kv [S, H, nope + v]`` and a key part ``k_rope [S, rope_dim]`` that
     the heads share (``None`` without one): ``[T, H, v]`` from ``q [T, H, nope + rope_dim]``.
 
     Sequences are packed: ``query_starts [B + 1]`` and ``kv_starts [B + 1]`` int32 (default: the same) bound their
     query tokens and keys, query starts as in :func:`absorbed_attention`. With ``causal`` query i of n sees the
     first ``keys - n + i + 1`` keys. ``nope`` and ``v`` are both 128 or both 64, ``rope_dim`` 64 or none. Keys and values
-    that a sequence's queries do not all see have to be finite; what no sequence holds may be anything. Empty rows,
-    ``return_lse`` and ``out`` as in :func:`absorbed_attention`.
+    that a sequence's queries do not all see have to be finite; what no sequence holds may be anything. With
+    ``window`` (and ``causal``) a query sees its last ``window`` keys, its own included, and the sequence's first
+    ``sinks``. Empty rows, ``return_lse`` and ``out`` as in :func:`absorbed_attention`.
     """
     o, lse = _native.require_native().latent_expanded_attention(q, kv, k_rope, query_starts, kv_starts, scale, causal,
-                                                                out, return_lse)
+                                                                out, return_lse, window, sinks)
     return (o, lse) if return_lse else o
 
 

@@ -327,6 +327,26 @@ typedef struct fcmoe_absorbed_args {
 size_t fcmoe_absorbed_attention_workspace_bytes(const fcmoe_absorbed_args* args);
 int fcmoe_absorbed_attention(const fcmoe_absorbed_args* args, hipStream_t stream);
 
+/* What a query row sees of a sequence beyond the causal rule. window > 0: a row
+ * at position p sees p - window + 1 .. p and the sequence's first `sinks`
+ * tokens (0: all before it). tree_masks (absorbed form): a sequence's last n
+ * tokens are its n query tokens, the nodes of a tree of drafts. Node i sees the
+ * tokens before them (of a window those that position len - n + depth sees) and
+ * of the nodes those j whose bit j % 64 of word j / 64 of its mask is set;
+ * nodes past the mask's words are not seen. No cached row outside what some row
+ * sees is read, but for copies of ones that are: its pages may be gone. Masks
+ * have 1 to 16 words a token, rows mask_stride words apart. */
+typedef struct fcmoe_key_mask {
+  int64_t window, sinks;
+  const uint64_t* tree_masks; /* [tokens, mask_words] or NULL */
+  int64_t mask_words, mask_stride;
+  const int32_t* tree_depths; /* [tokens] */
+} fcmoe_key_mask;
+/* As fcmoe_absorbed_attention (whose workspace is another's), for rows that see
+ * what `mask` says. */
+size_t fcmoe_absorbed_attention_masked_workspace_bytes(const fcmoe_absorbed_args* args, const fcmoe_key_mask* mask);
+int fcmoe_absorbed_attention_masked(const fcmoe_absorbed_args* args, const fcmoe_key_mask* mask, hipStream_t stream);
+
 /* Latent attention, expanded form: per-head keys and values kv [keys, heads,
  * nope_dim + v_dim] (keys, then values) and the key part k_rope [keys,
  * rope_dim] that the heads share; q [tokens, heads, nope_dim + rope_dim].
@@ -357,6 +377,81 @@ typedef struct fcmoe_expanded_args {
 } fcmoe_expanded_args;
 size_t fcmoe_expanded_attention_workspace_bytes(const fcmoe_expanded_args* args);
 int fcmoe_expanded_attention(const fcmoe_expanded_args* args, hipStream_t stream);
+/* As fcmoe_expanded_attention (whose workspace is another's), causal, for rows
+ * that see what `mask` says: its window and first tokens, no tree. */
+size_t fcmoe_expanded_attention_masked_workspace_bytes(const fcmoe_expanded_args* args, const fcmoe_key_mask* mask);
+int fcmoe_expanded_attention_masked(const fcmoe_expanded_args* args, const fcmoe_key_mask* mask, hipStream_t stream);
+
+/* Masks and depths of trees of drafted tokens, for fcmoe_key_mask: token i of
+ * sequence b (query_starts[b] .. [b + 1]) is a node whose parent is node
+ * parents[t] < i of the same sequence; any other value (-1) makes it a root. Bit j
+ * of masks [tokens, mask_words] is set for the node itself and its ancestors,
+ * depths [tokens] counts those. mask_words 1 to 16: nodes past 64 mask_words
+ * of a sequence, and tokens of none, get no bits and depth 0. */
+int fcmoe_draft_tree(const int32_t* parents, int64_t tokens, const int32_t* query_starts, int64_t batch, int64_t mask_words,
+                     uint64_t* masks, int32_t* depths, hipStream_t stream);
+
+/* What each cached token receives of the softmax weights of a call's query rows:
+ *   out[b, j] = previous[b, j] + sum exp(scale * (q_latent . c_j + q_rope . r_j) - lse[t, h])
+ * over the query tokens t of sequence b that see token j (as in
+ * fcmoe_absorbed_attention, whose lse [tokens, heads] is given) and their
+ * heads; for j < kv_lens[b], else previous[b, j]. out and previous (NULL: zeros) [batch,
+ * positions], rows out_stride and previous_stride values apart; out may be
+ * previous itself. Rows with an lse of -inf add nothing; a page id outside the
+ * cache makes its tokens' weights NaN. batch at most 65535. */
+typedef struct fcmoe_attention_weights_args {
+  const uint16_t* q_latent;
+  const uint16_t* q_rope;
+  int64_t tokens, heads, batch;
+  int64_t q_latent_token_stride, q_latent_head_stride;
+  int64_t q_rope_token_stride, q_rope_head_stride;
+  fcmoe_latent_cache cache;
+  const int32_t* page_table;
+  int64_t table_width, page_table_stride;
+  const int32_t* kv_lens;
+  const int32_t* query_starts;
+  const float* lse;
+  float scale;
+  const float* previous;
+  int64_t previous_stride;
+  float* out;
+  int64_t out_stride, positions;
+  void* workspace;
+  size_t workspace_bytes;
+} fcmoe_attention_weights_args;
+size_t fcmoe_attention_weights_workspace_bytes(const fcmoe_attention_weights_args* args);
+int fcmoe_attention_weights(const fcmoe_attention_weights_args* args, hipStream_t stream);
+
+/* The positions that stay when sequence b keeps `keep` of its kv_lens[b] tokens
+ * (cut to `positions`): all of them if there are no more, else its first
+ * `sinks`, its last `recent` and of the others those with the largest weights
+ * [batch, positions] (rows stride values apart), ties to the lower position, NaN
+ * as the largest. out_positions [batch, keep] ascends, -1 behind counts[b]; kept
+ * [batch, keep] has their weights, 0 behind. */
+int fcmoe_heaviest_positions(const float* weights, int64_t batch, int64_t positions, int64_t stride, const int32_t* kv_lens,
+                             int64_t keep, int64_t sinks, int64_t recent, int32_t* out_positions, int32_t* counts, float* kept,
+                             hipStream_t stream);
+
+/* Moves cached rows: row positions[b, k] of sequence b (page table [batch,
+ * table_width]) becomes its row starts[b] + k (starts NULL: k) for k < counts[b]
+ * <= most. With to_table the rows go to that table's pages, which hold no row
+ * that the call reads; without, they stay in their own: positions then ascend
+ * and positions[b, k] >= starts[b] + k, and no other sequence shares the pages
+ * that are written. A position without a cached row at either end is skipped. batch at
+ * most 65535. */
+typedef struct fcmoe_latent_move_args {
+  fcmoe_latent_cache cache;
+  const int32_t* page_table;
+  int64_t table_width, page_table_stride;
+  const int32_t* to_table;
+  int64_t to_width, to_stride;
+  const int32_t* positions;
+  int64_t most, positions_stride;
+  const int32_t* counts;
+  const int32_t* starts;
+  int64_t batch;
+} fcmoe_latent_move_args;
+int fcmoe_latent_cache_move(const fcmoe_latent_move_args* args, hipStream_t stream);
 
 /* ---- diagnostics (stage-level parity checks) ---------------------------- */
 
