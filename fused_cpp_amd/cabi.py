@@ -216,7 +216,8 @@ SIGNATURES = {
     "fcmoe_draft_tree": (_I, [_P, _I64, _P, _I64, _I64, _P, _P, _P]),
     "fcmoe_attention_weights_workspace_bytes": (_SZ, [ctypes.POINTER(AttentionWeightsArgs)]),
     "fcmoe_attention_weights": (_I, [ctypes.POINTER(AttentionWeightsArgs), _P]),
-    "fcmoe_heaviest_positions": (_I, [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _P]),
+    "fcmoe_heaviest_positions_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64]),
+    "fcmoe_heaviest_positions": (_I, [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _P, _SZ, _P]),
     "fcmoe_latent_cache_move": (_I, [ctypes.POINTER(LatentMoveArgs), _P]),
 }
 

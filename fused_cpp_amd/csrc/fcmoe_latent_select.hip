@@ -74,11 +74,21 @@ __global__ __launch_bounds__(kTreeThreads) void draft_tree_kernel(const Tree p) 
 // Of a sequence of len > keep tokens: its first `sinks`, its last `recent`, and of
 // the others the keep - sinks - recent with the largest weights, ties to the
 // lower position (NaN counts as the largest, -0 as 0), in ascending order.
-// A workgroup a sequence. The m-th largest weight is found from its bits, as
-// integers in the same order, 11, 11 and 10 at a time from the top: a histogram
-// in LDS of those that agree so far, then the bin that the m-th falls into. What
-// is kept is counted wave by wave and written in a second walk.
-constexpr int kHeavyWaves = 16, kBins = 2048, kCopies = 4;
+//
+// The m-th largest weight is found from its bits, as integers in the same
+// order, 11, 11 and 10 at a time from the top: a histogram in LDS of those that
+// agree so far, then the bin that the m-th falls into. What stays is counted wave
+// by wave and written in order.
+//
+// A workgroup holds kSlice weights in registers. Sequences of up to that many columns
+// are one launch, a workgroup each, that reads the weights once. Longer ones are cut into
+// slices, a workgroup each, in three launches (a CU alone takes some 10 bytes a
+// clock from memory): histograms of the first digit by slice; the weights of
+// the bin that they lead to, listed by slice; the other digits from those lists
+// (every workgroup for itself), and what stays of the slice behind what stays of
+// those before it.
+constexpr int kHeavyWaves = 16, kHeavyThreads = kHeavyWaves * kWave, kBins = 2048, kCopies = 4;
+constexpr int kHold = 8, kSlice = kHold * kHeavyThreads;
 
 struct Heavy {
   const float* weights;
@@ -89,6 +99,10 @@ struct Heavy {
   int32_t* out;  // [batch, keep], -1 behind the count
   int32_t* counts;
   float* kept;   // [batch, keep], 0 behind the count
+  int slices;    // of a sequence's columns; 1: one launch
+  int* hist;     // [batch, slices][kBins], first digits
+  uint32_t* list;  // [batch, slices][kSlice], the weights of the chosen bin, in their positions' order
+  int2* listed;    // [batch, slices]: weights above the bin, weights in it
 };
 
 __device__ __forceinline__ uint32_t order_of(float w) {
@@ -109,114 +123,308 @@ __device__ __forceinline__ int lanes_before(int v, int* total) {
   return upto - v;
 }
 
-__global__ __launch_bounds__(kHeavyWaves* kWave) void heaviest_kernel(const Heavy p) {
-  constexpr int THREADS = kHeavyWaves * kWave;
-  __shared__ int hist[kCopies][kBins];
-  __shared__ int waves[2][kHeavyWaves];
-  __shared__ int found[2];  // digit, how many of its bin
-  const int64_t b = blockIdx.x;
+struct HeavyLds {
+  int hist[kCopies][kBins];
+  int waves[2][kHeavyWaves];
+  int found[2];  // digit, how many of its bin
+};
+
+template <int COPIES>
+__device__ __forceinline__ void clear_bins(HeavyLds& l) {
+  for (int k = (int)threadIdx.x; k < COPIES * kBins; k += kHeavyThreads) l.hist[0][k] = 0;
+  __syncthreads();
+}
+// The bin that the need-th largest falls into, from the highest down; need becomes how many of that bin. The thread's
+// two bins hold n0 (bin 2047 - 2 thread) and n1 (the one below).
+__device__ __forceinline__ int pick_bin(HeavyLds& l, int n0, int n1, int& need) {
   const int tid = (int)threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  int total;
+  int before = lanes_before(n0 + n1, &total);
+  if (lane == 0) l.waves[0][wave] = total;
+  __syncthreads();
+  for (int v = 0; v < wave; ++v) before += l.waves[0][v];
+  if (before < need && before + n0 + n1 >= need) {
+    const bool upper = before + n0 >= need;
+    l.found[0] = kBins - 1 - 2 * tid - (upper ? 0 : 1);
+    l.found[1] = need - before - (upper ? 0 : n0);
+  }
+  __syncthreads();
+  need = l.found[1];
+  return l.found[0];
+}
+template <int COPIES>
+__device__ __forceinline__ int pick_bin(HeavyLds& l, int& need) {
+  __syncthreads();
+  const int hi = kBins - 1 - 2 * (int)threadIdx.x;
+  int n0 = 0, n1 = 0;
+#pragma unroll
+  for (int c = 0; c < COPIES; ++c) {
+    n0 += l.hist[c][hi];
+    n1 += l.hist[c][hi - 1];
+  }
+  return pick_bin(l, n0, n1, need);
+}
+
+// A sequence's span of weights that are compared, and how many of them stay (0: nothing to choose).
+struct HeavySpan {
+  int len, first, last, need;
+};
+__device__ __forceinline__ HeavySpan heavy_span(const Heavy& p, int64_t b) {
+  HeavySpan s;
+  s.len = (int)clamp64(p.lens[b], 0, p.positions);
+  s.first = p.sinks, s.last = s.len - p.recent;
+  s.need = s.len > p.keep ? (int)p.keep - p.sinks - p.recent : 0;
+  return s;
+}
+
+// Weight i of this thread among the slice from position `from` on: a wave has 64 kHold neighbours, 64 of them at a time.
+__device__ __forceinline__ int held_at(int from, int i) {
+  return from + ((int)threadIdx.x / kWave * kHold + i) * kWave + (int)threadIdx.x % kWave;
+}
+__device__ __forceinline__ void hold(const float* w, int from, int last, float (&v)[kHold]) {
+#pragma unroll
+  for (int i = 0; i < kHold; ++i) v[i] = held_at(from, i) < last ? w[held_at(from, i)] : 0.0f;
+}
+
+// Everything of a sequence but the weights that are compared.
+__device__ __forceinline__ void write_ends(const Heavy& p, int64_t b, const HeavySpan& s) {
+  const int tid = (int)threadIdx.x;
   const float* w = p.weights + b * p.stride;
   int32_t* out = p.out + b * p.keep;
   float* kept = p.kept + b * p.keep;
-  const int len = (int)clamp64(p.lens[b], 0, p.positions);
-  const int count = (int)(len < p.keep ? len : p.keep);
+  const int count = (int)(s.len < p.keep ? s.len : p.keep);
   if (tid == 0) p.counts[b] = count;
-  for (int64_t k = count + tid; k < p.keep; k += THREADS) {
+  for (int64_t k = count + tid; k < p.keep; k += kHeavyThreads) {
     out[k] = -1;
     kept[k] = 0.0f;
   }
-  if (len <= p.keep) {
-    for (int k = tid; k < len; k += THREADS) {
-      out[k] = k;
-      kept[k] = w[k];
-    }
-    return;
-  }
-  const int first = p.sinks, last = len - p.recent;  // the others: [first, last)
-  for (int k = tid; k < p.sinks; k += THREADS) {
+  const int head = s.len > p.keep ? p.sinks : s.len;
+  for (int k = tid; k < head; k += kHeavyThreads) {
     out[k] = k;
     kept[k] = w[k];
   }
-  for (int k = tid; k < p.recent; k += THREADS) {
-    out[p.keep - p.recent + k] = last + k;
-    kept[p.keep - p.recent + k] = w[last + k];
+  if (s.len <= p.keep) return;
+  for (int k = tid; k < p.recent; k += kHeavyThreads) {
+    out[p.keep - p.recent + k] = s.last + k;
+    kept[p.keep - p.recent + k] = w[s.last + k];
   }
-  int need = (int)p.keep - p.sinks - p.recent;
-  if (need <= 0) return;
+}
 
-  uint32_t prefix = 0, mask = 0;
-#pragma unroll
-  for (int round = 0; round < 3; ++round) {
-    const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
-    const uint32_t digits = round == 2 ? 1023u : 2047u;
-    for (int k = tid; k < kCopies * kBins; k += THREADS) hist[k / kBins][k % kBins] = 0;
-    __syncthreads();
-    for (int j = first + tid; j < last; j += THREADS) {
-      const uint32_t u = order_of(w[j]);
-      if ((u & mask) == prefix) atomicAdd(&hist[wave % kCopies][u >> shift & digits], 1);
-    }
-    __syncthreads();
-    // thread t has bins 2047 - 2 t and the one below: the largest first
-    const int hi = kBins - 1 - 2 * tid;
-    int n0 = 0, n1 = 0;
-#pragma unroll
-    for (int c = 0; c < kCopies; ++c) {
-      n0 += hist[c][hi];
-      n1 += hist[c][hi - 1];
-    }
-    int total;
-    int before = lanes_before(n0 + n1, &total);
-    if (lane == 0) waves[0][wave] = total;
-    __syncthreads();
-    for (int v = 0; v < wave; ++v) before += waves[0][v];
-    if (before < need && before + n0 + n1 >= need) {
-      const bool upper = before + n0 >= need;
-      found[0] = upper ? hi : hi - 1;
-      found[1] = need - before - (upper ? 0 : n0);
-    }
-    __syncthreads();
-    prefix |= (uint32_t)found[0] << shift;
-    mask |= digits << shift;
-    need = found[1];
-  }
-  // what is above `prefix` stays, and the first `need` that equal it
-  const int blocks = (last - first + kWave - 1) / kWave;  // 64 positions each, in turn to the waves
-  const int k0 = (int)((int64_t)blocks * wave / kHeavyWaves), k1 = (int)((int64_t)blocks * (wave + 1) / kHeavyWaves);
+// Writes the held weights above `bound` and the first of those that equal it, `need` less the `ties` before this
+// slice, from place `at` on.
+__device__ __forceinline__ void write_kept(HeavyLds& l, const Heavy& p, int64_t b, const float (&v)[kHold], int from, int last,
+                                           uint32_t bound, int need, int ties, int at) {
+  const int lane = (int)threadIdx.x % kWave, wave = (int)threadIdx.x / kWave;
   int above = 0, same = 0;
-  for (int k = k0; k < k1; ++k) {
-    const int j = first + k * kWave + lane;
-    const uint32_t u = j < last ? order_of(w[j]) : 0;
-    above += __popcll(__ballot(j < last && u > prefix));
-    same += __popcll(__ballot(j < last && u == prefix));
+#pragma unroll
+  for (int i = 0; i < kHold; ++i) {
+    const bool in = held_at(from, i) < last;
+    const uint32_t u = order_of(v[i]);
+    above += __popcll(__ballot(in && u > bound));
+    same += __popcll(__ballot(in && u == bound));
   }
   if (lane == 0) {
-    waves[0][wave] = above;
-    waves[1][wave] = same;
+    l.waves[0][wave] = above;
+    l.waves[1][wave] = same;
   }
   __syncthreads();
-  int at = p.sinks, ties = 0;  // places taken before this wave's, ties among the positions before
-  for (int v = 0; v < wave; ++v) {
-    const int s = waves[1][v], stay = max(min(need - ties, s), 0);
-    at += waves[0][v] + stay;
+  for (int k = 0; k < wave; ++k) {
+    const int s = l.waves[1][k];
+    at += l.waves[0][k] + max(min(need - ties, s), 0);
     ties += s;
   }
   const uint64_t lower = ((uint64_t)1 << lane) - 1;
-  for (int k = k0; k < k1; ++k) {
-    const int j = first + k * kWave + lane;
-    const float v = j < last ? w[j] : 0.0f;
-    const uint32_t u = order_of(v);
-    const uint64_t eq = __ballot(j < last && u == prefix);
-    const bool stays = j < last && (u > prefix || (u == prefix && ties + __popcll(eq & lower) < need));
+#pragma unroll
+  for (int i = 0; i < kHold; ++i) {
+    const int j = held_at(from, i);
+    const uint32_t u = order_of(v[i]);
+    const uint64_t eq = __ballot(j < last && u == bound);
+    const bool stays = j < last && (u > bound || (u == bound && ties + __popcll(eq & lower) < need));
     const uint64_t all = __ballot(stays);
     if (stays) {
-      const int to = at + __popcll(all & lower);
-      out[to] = j;
-      kept[to] = v;
+      const int64_t to = b * p.keep + at + __popcll(all & lower);
+      p.out[to] = j;
+      p.kept[to] = v[i];
     }
     at += __popcll(all);
     ties += __popcll(eq);
   }
+}
+
+__global__ __launch_bounds__(kHeavyThreads) void heaviest_kernel(const Heavy p) {
+  __shared__ HeavyLds l;
+  const int64_t b = blockIdx.x;
+  const int wave = (int)threadIdx.x / kWave;
+  const HeavySpan s = heavy_span(p, b);
+  float v[kHold];
+  if (s.need > 0) hold(p.weights + b * p.stride, s.first, s.last, v);
+  write_ends(p, b, s);
+  if (s.need <= 0) return;
+  int need = s.need;
+  uint32_t bound = 0, mask = 0;
+#pragma unroll
+  for (int round = 0; round < 3; ++round) {
+    const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
+    const uint32_t digits = round == 2 ? 1023u : 2047u;
+    clear_bins<kCopies>(l);
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) {
+      const uint32_t u = order_of(v[i]);
+      if (held_at(s.first, i) < s.last && (u & mask) == bound) atomicAdd(&l.hist[wave % kCopies][u >> shift & digits], 1);
+    }
+    bound |= (uint32_t)pick_bin<kCopies>(l, need) << shift;
+    mask |= digits << shift;
+  }
+  write_kept(l, p, b, v, s.first, s.last, bound, need, 0, p.sinks);
+}
+
+// The first digits of a slice.
+__global__ __launch_bounds__(kHeavyThreads) void heaviest_count_kernel(const Heavy p) {
+  __shared__ HeavyLds l;
+  const int64_t b = blockIdx.y;
+  const int wave = (int)threadIdx.x / kWave;
+  const HeavySpan s = heavy_span(p, b);
+  const int from = s.first + (int)blockIdx.x * kSlice;
+  if (blockIdx.x == 0) write_ends(p, b, s);
+  if (s.need <= 0 || from >= s.last) return;
+  float v[kHold];
+  hold(p.weights + b * p.stride, from, s.last, v);
+  clear_bins<kCopies>(l);
+#pragma unroll
+  for (int i = 0; i < kHold; ++i)
+    if (held_at(from, i) < s.last) atomicAdd(&l.hist[wave % kCopies][order_of(v[i]) >> 21], 1);
+  __syncthreads();
+  int* to = p.hist + (b * p.slices + blockIdx.x) * kBins;
+  for (int k = (int)threadIdx.x; k < kBins; k += kHeavyThreads) {
+    int n = 0;
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) n += l.hist[c][k];
+    to[k] = n;
+  }
+}
+
+// The bin of the first digit, from all slices' histograms.
+__device__ __forceinline__ uint32_t first_digit(HeavyLds& l, const Heavy& p, int64_t b, const HeavySpan& s, int& need) {
+  const int used = (s.last - s.first + kSlice - 1) / kSlice, hi = kBins - 1 - 2 * (int)threadIdx.x;
+  const int* h = p.hist + b * p.slices * kBins + hi - 1;
+  int n0 = 0, n1 = 0;
+#pragma unroll 4
+  for (int k = 0; k < used; ++k) {
+    const int2 n = *(const int2*)(h + (int64_t)k * kBins);
+    n1 += n.x;
+    n0 += n.y;
+  }
+  return (uint32_t)pick_bin(l, n0, n1, need);
+}
+
+__global__ __launch_bounds__(kHeavyThreads) void heaviest_list_kernel(const Heavy p) {
+  __shared__ HeavyLds l;
+  const int64_t b = blockIdx.y;
+  const int lane = (int)threadIdx.x % kWave, wave = (int)threadIdx.x / kWave;
+  const HeavySpan s = heavy_span(p, b);
+  const int from = s.first + (int)blockIdx.x * kSlice;
+  if (s.need <= 0 || from >= s.last) return;
+  float v[kHold];
+  hold(p.weights + b * p.stride, from, s.last, v);
+  int need = s.need;
+  const uint32_t digit = first_digit(l, p, b, s, need);
+  int above = 0, in_bin = 0;
+#pragma unroll
+  for (int i = 0; i < kHold; ++i) {
+    const bool in = held_at(from, i) < s.last;
+    const uint32_t d = order_of(v[i]) >> 21;
+    above += __popcll(__ballot(in && d > digit));
+    in_bin += __popcll(__ballot(in && d == digit));
+  }
+  __syncthreads();
+  if (lane == 0) {
+    l.waves[0][wave] = above;
+    l.waves[1][wave] = in_bin;
+  }
+  __syncthreads();
+  int at = 0, all_above = 0, all = 0;
+  for (int k = 0; k < kHeavyWaves; ++k) {
+    if (k < wave) at += l.waves[1][k];
+    all_above += l.waves[0][k];
+    all += l.waves[1][k];
+  }
+  const int64_t slice = b * p.slices + blockIdx.x;
+  if (threadIdx.x == 0) p.listed[slice] = make_int2(all_above, all);
+  uint32_t* to = p.list + slice * kSlice;
+#pragma unroll
+  for (int i = 0; i < kHold; ++i) {
+    const uint32_t u = order_of(v[i]);
+    const bool in = held_at(from, i) < s.last && u >> 21 == digit;
+    const uint64_t which = __ballot(in);
+    if (in) to[at + __popcll(which & (((uint64_t)1 << lane) - 1))] = u;
+    at += __popcll(which);
+  }
+}
+
+__global__ __launch_bounds__(kHeavyThreads) void heaviest_write_kernel(const Heavy p) {
+  __shared__ HeavyLds l;
+  __shared__ int sums[2];
+  const int64_t b = blockIdx.y;
+  const int tid = (int)threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const HeavySpan s = heavy_span(p, b);
+  const int from = s.first + (int)blockIdx.x * kSlice;
+  if (s.need <= 0 || from >= s.last) return;
+  float v[kHold];
+  hold(p.weights + b * p.stride, from, s.last, v);
+  const int used = (s.last - s.first + kSlice - 1) / kSlice;
+  const int2* listed = p.listed + b * p.slices;
+  int need = s.need;
+  uint32_t bound = first_digit(l, p, b, s, need) << 21, mask = 2047u << 21;
+  // a wave a slice's list, and more of them where it is long
+  auto each = [&](int slices, auto f) {
+    for (int k = 0; k < slices; ++k) {
+      const uint32_t* list = p.list + (b * p.slices + k) * kSlice;
+      const int n = listed[k].y;
+      for (int i = (tid + (k * 2 + 1) * (kHeavyThreads / 2)) % kHeavyThreads; i < n; i += kHeavyThreads) f(list[i]);
+    }
+  };
+#pragma unroll
+  for (int round = 1; round < 3; ++round) {
+    const int shift = round == 1 ? 10 : 0;
+    const uint32_t digits = round == 2 ? 1023u : 2047u;
+    clear_bins<kCopies>(l);
+    each(used, [&](uint32_t u) {
+      if ((u & mask) == bound) atomicAdd(&l.hist[wave % kCopies][u >> shift & digits], 1);
+    });
+    bound |= (uint32_t)pick_bin<kCopies>(l, need) << shift;
+    mask |= digits << shift;
+  }
+  // what stays of the slices before this one
+  if (tid < 2) sums[tid] = 0;
+  __syncthreads();
+  int above = 0, same = 0;
+  each((int)blockIdx.x, [&](uint32_t u) {
+    above += u > bound;
+    same += u == bound;
+  });
+  for (int k = tid; k < (int)blockIdx.x; k += kHeavyThreads) above += listed[k].x;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    above += __shfl_xor(above, o);
+    same += __shfl_xor(same, o);
+  }
+  if (lane == 0) {
+    atomicAdd(&sums[0], above);
+    atomicAdd(&sums[1], same);
+  }
+  __syncthreads();
+  write_kept(l, p, b, v, from, s.last, bound, need, sums[1], p.sinks + sums[0] + min(need, sums[1]));
+}
+
+int heavy_slices(int64_t positions) { return (int)ceil_div(positions > 0 ? positions : 1, kSlice); }
+size_t heavy_list_bytes(int64_t batch, int64_t slices) { return (size_t)batch * (size_t)slices * kSlice * 4; }
+size_t heavy_hist_bytes(int64_t batch, int64_t slices) { return (size_t)batch * (size_t)slices * kBins * 4; }
+
+int check_heavy(int64_t batch, int64_t positions, int64_t stride, int64_t keep, int64_t sinks, int64_t recent) {
+  if (batch < 0 || batch > 65535 || positions < 0 || positions > INT32_MAX - 4 * kSlice || stride < 0 || keep < 1 || keep > INT32_MAX - 4096 ||
+      sinks < 0 || recent < 0 || sinks > keep || recent > keep - sinks)
+    return fail(FCMOE_EINVAL, "heaviest_positions: bad shape (keep at least 1, and no fewer than sinks + recent)");
+  return FCMOE_OK;
 }
 
 // ---- moving cached rows ---------------------------------------------------------
@@ -355,17 +563,38 @@ extern "C" int fcmoe_draft_tree(const int32_t* parents, int64_t tokens, const in
   return check_launch("draft_tree");
 }
 
+extern "C" size_t fcmoe_heaviest_positions_workspace_bytes(int64_t batch, int64_t positions, int64_t keep, int64_t sinks, int64_t recent) {
+  if (check_heavy(batch, positions, 0, keep, sinks, recent) != FCMOE_OK || batch == 0) return 0;
+  const int64_t slices = heavy_slices(positions);
+  return slices == 1 ? 0 : heavy_list_bytes(batch, slices) + heavy_hist_bytes(batch, slices) + (size_t)batch * (size_t)slices * 8;
+}
+
 extern "C" int fcmoe_heaviest_positions(const float* weights, int64_t batch, int64_t positions, int64_t stride,
                                         const int32_t* kv_lens, int64_t keep, int64_t sinks, int64_t recent,
-                                        int32_t* out_positions, int32_t* counts, float* kept, hipStream_t stream) {
-  if (batch < 0 || batch > (1 << 20) || positions < 0 || positions > INT32_MAX - 4096 || stride < 0 || keep < 1 || keep > INT32_MAX - 4096 ||
-      sinks < 0 || recent < 0 || sinks > keep || recent > keep - sinks)
-    return fail(FCMOE_EINVAL, "heaviest_positions: bad shape (keep at least 1, and no fewer than sinks + recent)");
+                                        int32_t* out_positions, int32_t* counts, float* kept, void* workspace,
+                                        size_t workspace_bytes, hipStream_t stream) {
+  if (const int rc = check_heavy(batch, positions, stride, keep, sinks, recent)) return rc;
   if (batch == 0) return FCMOE_OK;
   if ((positions > 0 && !weights) || !kv_lens || !out_positions || !counts || !kept)
     return fail(FCMOE_EINVAL, "heaviest_positions: NULL pointer");
-  Heavy p{weights, positions, stride, kv_lens, keep, (int)sinks, (int)recent, out_positions, counts, kept};
-  hipLaunchKernelGGL(heaviest_kernel, dim3((unsigned)batch), dim3(kHeavyWaves * kWave), 0, stream, p);
+  Heavy p{};
+  p.weights = weights, p.positions = positions, p.stride = stride, p.lens = kv_lens, p.keep = keep;
+  p.sinks = (int)sinks, p.recent = (int)recent, p.out = out_positions, p.counts = counts, p.kept = kept;
+  p.slices = heavy_slices(positions);
+  if (p.slices == 1) {
+    hipLaunchKernelGGL(heaviest_kernel, dim3((unsigned)batch), dim3(kHeavyThreads), 0, stream, p);
+    return check_launch("heaviest_positions");
+  }
+  if (!workspace || workspace_bytes < fcmoe_heaviest_positions_workspace_bytes(batch, positions, keep, sinks, recent))
+    return fail(FCMOE_ESPACE, "heaviest_positions: workspace too small");
+  if ((uintptr_t)workspace % 16) return fail(FCMOE_EINVAL, "heaviest_positions: unaligned workspace");
+  p.list = (uint32_t*)workspace;
+  p.hist = (int*)((char*)workspace + heavy_list_bytes(batch, p.slices));
+  p.listed = (int2*)((char*)p.hist + heavy_hist_bytes(batch, p.slices));
+  const dim3 g((unsigned)p.slices, (unsigned)batch), t(kHeavyThreads);
+  hipLaunchKernelGGL(heaviest_count_kernel, g, t, 0, stream, p);
+  hipLaunchKernelGGL(heaviest_list_kernel, g, t, 0, stream, p);
+  hipLaunchKernelGGL(heaviest_write_kernel, g, t, 0, stream, p);
   return check_launch("heaviest_positions");
 }
 

@@ -775,7 +775,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> heaviest_positions(at::Tensor wei
   TORCH_CHECK_VALUE(keep >= 1 && keep <= INT32_MAX - 4096, "keep must be at least 1, got ", keep);
   TORCH_CHECK_VALUE(sinks >= 0 && recent >= 0 && sinks <= keep && recent <= keep - sinks,
                     "sinks and recent must not be negative, nor more than keep together: got ", sinks, ", ", recent, " of ", keep);
-  TORCH_CHECK_VALUE(B <= (1 << 20) && S <= INT32_MAX - 4096, "too many sequences or positions");
+  TORCH_CHECK_VALUE(B <= 65535 && S <= INT32_MAX - (1 << 16), "too many sequences or positions");
   check_no_grad({&weights}, what);
   check_devices(weights, {&kv_lens}, what);
   c10::DeviceGuard guard(weights.device());
@@ -783,10 +783,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> heaviest_positions(at::Tensor wei
   at::Tensor positions = at::empty({B, keep}, ints), counts = at::empty({B}, ints), kept = at::empty({B, keep}, weights.options());
   if (B == 0) return {positions, counts, kept};
   const at::Tensor w = weight_rows_ok(weights) ? weights : weights.contiguous(), lens = kv_lens.contiguous();
+  const size_t bytes = fcmoe_heaviest_positions_workspace_bytes(B, S, keep, sinks, recent);
+  at::Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes}, weights.options().dtype(at::kByte));
   {
     pybind11::gil_scoped_release release;
     check_rc(fcmoe_heaviest_positions(w.data_ptr<float>(), B, S, stride_at(w, 0), lens.data_ptr<int32_t>(), keep, sinks, recent,
-                                      positions.data_ptr<int32_t>(), counts.data_ptr<int32_t>(), kept.data_ptr<float>(), stream_of(weights)),
+                                      positions.data_ptr<int32_t>(), counts.data_ptr<int32_t>(), kept.data_ptr<float>(),
+                                      bytes ? ws.data_ptr() : nullptr, bytes, stream_of(weights)),
              what);
   }
   return {positions, counts, kept};

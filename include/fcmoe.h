@@ -427,10 +427,11 @@ int fcmoe_attention_weights(const fcmoe_attention_weights_args* args, hipStream_
  * `sinks`, its last `recent` and of the others those with the largest weights
  * [batch, positions] (rows stride values apart), ties to the lower position, NaN
  * as the largest. out_positions [batch, keep] ascends, -1 behind counts[b]; kept
- * [batch, keep] has their weights, 0 behind. */
+ * [batch, keep] has their weights, 0 behind. batch at most 65535. */
+size_t fcmoe_heaviest_positions_workspace_bytes(int64_t batch, int64_t positions, int64_t keep, int64_t sinks, int64_t recent);
 int fcmoe_heaviest_positions(const float* weights, int64_t batch, int64_t positions, int64_t stride, const int32_t* kv_lens,
                              int64_t keep, int64_t sinks, int64_t recent, int32_t* out_positions, int32_t* counts, float* kept,
-                             hipStream_t stream);
+                             void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 /* Moves cached rows: row positions[b, k] of sequence b (page table [batch,
  * table_width]) becomes its row starts[b] + k (starts NULL: k) for k < counts[b]

@@ -29,7 +29,7 @@ def _check_heaviest(w, lens, keep, sinks, recent):
         assert bool((got[len(want):] == 0).all())
 
 
-@pytest.mark.parametrize("S", [1, 63, 64, 65, 1000, 5000, 40000])
+@pytest.mark.parametrize("S", [1, 63, 64, 65, 1000, 5000, 8192, 8193, 40000])
 @pytest.mark.parametrize("kind", ["heavy", "ties", "zeros", "signs"])
 def test_heaviest_matches(gpu, S, kind):
     """Weights as they build up, with many ties, all alike, of both signs with both zeros; counts from 1 to all."""
@@ -68,6 +68,23 @@ def test_heaviest_lengths_and_strides(gpu):
     assert e[0].shape == (0, 3)
     z = lc.heaviest_positions(torch.zeros((2, 0), device="cuda"), _i32([4, 0]), 3)
     assert z[0].tolist() == [[-1] * 3] * 2 and z[1].tolist() == [0, 0] and z[2].tolist() == [[0.0] * 3] * 2
+
+
+def test_heaviest_of_many_slices(gpu):
+    """Long rows: all weights alike, alike but for a few, in one bin of the first digit, and spread; the slices before the
+    last that stays empty of what is kept, or full of it."""
+    S = 70000
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = torch.rand((5, S), generator=g, device="cuda")
+    w[0] = 0.5
+    w[1] = 0.0
+    w[1, 30000:30100] = torch.rand(100, generator=g, device="cuda")
+    w[2] = 1 + w[2] * 1e-3
+    w[3, :20000] += 1000
+    w[4, -9000:] += 1000
+    for lens in ([S] * 5, [S - 1, 50000, 8193, 24577, 66000]):
+        for keep, sinks, recent in ((1, 0, 0), (9000, 4, 64), (9000, 8990, 10), (20000, 0, 0), (69999, 1, 1), (69000, 9000, 9000)):
+            _check_heaviest(w, lens, keep, sinks, recent)
 
 
 def test_heaviest_many_sequences(gpu):

@@ -264,12 +264,17 @@ def test_cabi_refusals():
     for tokens, batch, words in ((-1, 1, 1), (1, 0, 1), (1, 1, 0), (1, 1, 17), (1 << 40, 1, 1)):
         _err(L.fcmoe_draft_tree(4096, tokens, 4096, batch, words, 4096, 4096, None), -1, b"bad shape")
     heavy = lambda **kw: [{**dict(w=4096, batch=2, positions=9, stride=9, lens=4096, keep=4, sinks=1, recent=1, o=4096, c=4096,  # noqa: E731
-                                  k=4096, s=None), **kw}[n] for n in ("w", "batch", "positions", "stride", "lens", "keep", "sinks",
-                                                                      "recent", "o", "c", "k", "s")]
+                                  k=4096, ws=None, nb=0, s=None), **kw}[n]
+                         for n in ("w", "batch", "positions", "stride", "lens", "keep", "sinks", "recent", "o", "c", "k", "ws", "nb", "s")]
     for bad in ({"keep": 0}, {"sinks": -1}, {"recent": -1}, {"sinks": 4}, {"positions": -1}, {"positions": 1 << 40}, {"batch": -1}):
         _err(L.fcmoe_heaviest_positions(*heavy(**bad)), -1, b"bad shape")
     _err(L.fcmoe_heaviest_positions(*heavy(w=None)), -1, b"NULL pointer")
     assert L.fcmoe_heaviest_positions(*heavy(batch=0)) == 0
+    assert L.fcmoe_heaviest_positions_workspace_bytes(2, 8192, 4, 1, 1) == 0
+    need = L.fcmoe_heaviest_positions_workspace_bytes(2, 8193, 4, 1, 1)
+    assert need > 2 * 2 * 8192 * 4
+    _err(L.fcmoe_heaviest_positions(*heavy(positions=8193, ws=4096, nb=need - 1)), -2, b"workspace")
+    _err(L.fcmoe_heaviest_positions(*heavy(positions=8193, ws=4100, nb=need)), -1, b"unaligned")
     w = cabi.AttentionWeightsArgs(tokens=2, heads=1, batch=1, scale=1.0, cache=_desc())
     _err(L.fcmoe_attention_weights(w, None), -1, b"query_starts")
     w.batch, w.scale, w.positions = 2, -1.0, 10
