@@ -84,10 +84,14 @@ __global__ __launch_bounds__(kTreeThreads) void draft_tree_kernel(const Tree p) 
 // are one launch, a workgroup each, that reads the weights once. Longer ones are cut into
 // slices, a workgroup each, in three launches (a CU alone takes some 10 bytes a
 // clock from memory): histograms of the first digit by slice; the weights of
-// the bin that they lead to, listed by slice; the other digits from those lists
-// (every workgroup for itself), and what stays of the slice behind what stays of
-// those before it.
-constexpr int kHeavyWaves = 16, kHeavyThreads = kHeavyWaves * kWave, kBins = 2048, kCopies = 4;
+// the bin that they lead to, in one list (the histograms say where a slice's
+// begin); the other digits from that list, every workgroup for itself, and what
+// stays of the slice behind what stays of those before it.
+constexpr int kHeavyWaves = 16, kHeavyThreads = kHeavyWaves * kWave, kBins = 2048;
+// Histograms of the three digits, several of each that waves share: many weights have one first digit.
+constexpr int kCopies = 8;
+__device__ constexpr int copy_of(int round) { return round == 0 ? 0 : 2 + 2 * round; }
+__device__ constexpr int copies_of(int round) { return round == 0 ? 4 : 2; }
 constexpr int kHold = 8, kSlice = kHold * kHeavyThreads;
 
 struct Heavy {
@@ -100,9 +104,8 @@ struct Heavy {
   int32_t* counts;
   float* kept;   // [batch, keep], 0 behind the count
   int slices;    // of a sequence's columns; 1: one launch
-  int* hist;     // [batch, slices][kBins], first digits
-  uint32_t* list;  // [batch, slices][kSlice], the weights of the chosen bin, in their positions' order
-  int2* listed;    // [batch, slices]: weights above the bin, weights in it
+  int* hist;       // [batch, slices][kBins], first digits
+  uint32_t* list;  // [batch][slices * kSlice], the weights of the chosen bin, in their positions' order
 };
 
 __device__ __forceinline__ uint32_t order_of(float w) {
@@ -124,14 +127,13 @@ __device__ __forceinline__ int lanes_before(int v, int* total) {
 }
 
 struct HeavyLds {
-  int hist[kCopies][kBins];
+  alignas(16) int hist[kCopies][kBins];
   int waves[2][kHeavyWaves];
   int found[2];  // digit, how many of its bin
 };
 
-template <int COPIES>
 __device__ __forceinline__ void clear_bins(HeavyLds& l) {
-  for (int k = (int)threadIdx.x; k < COPIES * kBins; k += kHeavyThreads) l.hist[0][k] = 0;
+  for (int k = (int)threadIdx.x; k < kCopies * kBins / 4; k += kHeavyThreads) ((int4*)l.hist[0])[k] = make_int4(0, 0, 0, 0);
   __syncthreads();
 }
 // The bin that the need-th largest falls into, from the highest down; need becomes how many of that bin. The thread's
@@ -152,17 +154,20 @@ __device__ __forceinline__ int pick_bin(HeavyLds& l, int n0, int n1, int& need) 
   need = l.found[1];
   return l.found[0];
 }
-template <int COPIES>
-__device__ __forceinline__ int pick_bin(HeavyLds& l, int& need) {
+__device__ __forceinline__ int pick_bin(HeavyLds& l, int round, int& need) {
   __syncthreads();
-  const int hi = kBins - 1 - 2 * (int)threadIdx.x;
+  const int lo = kBins - 2 - 2 * (int)threadIdx.x;
   int n0 = 0, n1 = 0;
 #pragma unroll
-  for (int c = 0; c < COPIES; ++c) {
-    n0 += l.hist[c][hi];
-    n1 += l.hist[c][hi - 1];
+  for (int c = 0; c < copies_of(round); ++c) {
+    const int2 n = *(const int2*)&l.hist[copy_of(round) + c][lo];
+    n1 += n.x;
+    n0 += n.y;
   }
   return pick_bin(l, n0, n1, need);
+}
+__device__ __forceinline__ void add_to_bin(HeavyLds& l, int round, uint32_t digit) {
+  atomicAdd(&l.hist[copy_of(round) + (int)threadIdx.x / kWave % copies_of(round)][digit], 1);
 }
 
 // A sequence's span of weights that are compared, and how many of them stay (0: nothing to choose).
@@ -254,10 +259,10 @@ __device__ __forceinline__ void write_kept(HeavyLds& l, const Heavy& p, int64_t 
 __global__ __launch_bounds__(kHeavyThreads) void heaviest_kernel(const Heavy p) {
   __shared__ HeavyLds l;
   const int64_t b = blockIdx.x;
-  const int wave = (int)threadIdx.x / kWave;
   const HeavySpan s = heavy_span(p, b);
   float v[kHold];
   if (s.need > 0) hold(p.weights + b * p.stride, s.first, s.last, v);
+  if (s.need > 0) clear_bins(l);
   write_ends(p, b, s);
   if (s.need <= 0) return;
   int need = s.need;
@@ -266,13 +271,12 @@ __global__ __launch_bounds__(kHeavyThreads) void heaviest_kernel(const Heavy p) 
   for (int round = 0; round < 3; ++round) {
     const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
     const uint32_t digits = round == 2 ? 1023u : 2047u;
-    clear_bins<kCopies>(l);
 #pragma unroll
     for (int i = 0; i < kHold; ++i) {
       const uint32_t u = order_of(v[i]);
-      if (held_at(s.first, i) < s.last && (u & mask) == bound) atomicAdd(&l.hist[wave % kCopies][u >> shift & digits], 1);
+      if (held_at(s.first, i) < s.last && (u & mask) == bound) add_to_bin(l, round, u >> shift & digits);
     }
-    bound |= (uint32_t)pick_bin<kCopies>(l, need) << shift;
+    bound |= (uint32_t)pick_bin(l, round, need) << shift;
     mask |= digits << shift;
   }
   write_kept(l, p, b, v, s.first, s.last, bound, need, 0, p.sinks);
@@ -282,39 +286,56 @@ __global__ __launch_bounds__(kHeavyThreads) void heaviest_kernel(const Heavy p) 
 __global__ __launch_bounds__(kHeavyThreads) void heaviest_count_kernel(const Heavy p) {
   __shared__ HeavyLds l;
   const int64_t b = blockIdx.y;
-  const int wave = (int)threadIdx.x / kWave;
   const HeavySpan s = heavy_span(p, b);
   const int from = s.first + (int)blockIdx.x * kSlice;
   if (blockIdx.x == 0) write_ends(p, b, s);
   if (s.need <= 0 || from >= s.last) return;
   float v[kHold];
   hold(p.weights + b * p.stride, from, s.last, v);
-  clear_bins<kCopies>(l);
+  clear_bins(l);
 #pragma unroll
   for (int i = 0; i < kHold; ++i)
-    if (held_at(from, i) < s.last) atomicAdd(&l.hist[wave % kCopies][order_of(v[i]) >> 21], 1);
+    if (held_at(from, i) < s.last) add_to_bin(l, 0, order_of(v[i]) >> 21);
   __syncthreads();
   int* to = p.hist + (b * p.slices + blockIdx.x) * kBins;
   for (int k = (int)threadIdx.x; k < kBins; k += kHeavyThreads) {
     int n = 0;
 #pragma unroll
-    for (int c = 0; c < kCopies; ++c) n += l.hist[c][k];
+    for (int c = 0; c < copies_of(0); ++c) n += l.hist[copy_of(0) + c][k];
     to[k] = n;
   }
 }
 
-// The bin of the first digit, from all slices' histograms.
-__device__ __forceinline__ uint32_t first_digit(HeavyLds& l, const Heavy& p, int64_t b, const HeavySpan& s, int& need) {
-  const int used = (s.last - s.first + kSlice - 1) / kSlice, hi = kBins - 1 - 2 * (int)threadIdx.x;
-  const int* h = p.hist + b * p.slices * kBins + hi - 1;
-  int n0 = 0, n1 = 0;
-#pragma unroll 4
+// The bin of the first digit from all slices' histograms, and what those say of the weights in it and above it.
+struct FirstDigit {
+  uint32_t digit;
+  int above, before, all;  // weights above the bin in the slices before this one; in the bin there, in all slices
+};
+__device__ __forceinline__ FirstDigit first_digit(HeavyLds& l, const Heavy& p, int64_t b, const HeavySpan& s, int& need) {
+  __shared__ int sums[3];
+  const int used = (s.last - s.first + kSlice - 1) / kSlice, lo = kBins - 2 - 2 * (int)threadIdx.x;
+  const int* h = p.hist + b * p.slices * kBins + lo;
+  int n0 = 0, n1 = 0, m0 = 0, m1 = 0;
+#pragma unroll 8
   for (int k = 0; k < used; ++k) {
     const int2 n = *(const int2*)(h + (int64_t)k * kBins);
     n1 += n.x;
     n0 += n.y;
+    m1 += k < (int)blockIdx.x ? n.x : 0;
+    m0 += k < (int)blockIdx.x ? n.y : 0;
   }
-  return (uint32_t)pick_bin(l, n0, n1, need);
+  if (threadIdx.x < 3) sums[threadIdx.x] = 0;
+  const int digit = pick_bin(l, n0, n1, need);
+  int above = (lo + 1 > digit ? m0 : 0) + (lo > digit ? m1 : 0);
+  if (lo == digit || lo + 1 == digit) {
+    sums[1] = lo == digit ? m1 : m0;
+    sums[2] = lo == digit ? n1 : n0;
+  }
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) above += __shfl_xor(above, o);
+  if ((int)threadIdx.x % kWave == 0 && above) atomicAdd(&sums[0], above);
+  __syncthreads();
+  return FirstDigit{(uint32_t)digit, sums[0], sums[1], sums[2]};
 }
 
 __global__ __launch_bounds__(kHeavyThreads) void heaviest_list_kernel(const Heavy p) {
@@ -327,34 +348,19 @@ __global__ __launch_bounds__(kHeavyThreads) void heaviest_list_kernel(const Heav
   float v[kHold];
   hold(p.weights + b * p.stride, from, s.last, v);
   int need = s.need;
-  const uint32_t digit = first_digit(l, p, b, s, need);
-  int above = 0, in_bin = 0;
+  const FirstDigit f = first_digit(l, p, b, s, need);
+  int in_bin = 0;
 #pragma unroll
-  for (int i = 0; i < kHold; ++i) {
-    const bool in = held_at(from, i) < s.last;
-    const uint32_t d = order_of(v[i]) >> 21;
-    above += __popcll(__ballot(in && d > digit));
-    in_bin += __popcll(__ballot(in && d == digit));
-  }
+  for (int i = 0; i < kHold; ++i) in_bin += __popcll(__ballot(held_at(from, i) < s.last && order_of(v[i]) >> 21 == f.digit));
+  if (lane == 0) l.waves[1][wave] = in_bin;
   __syncthreads();
-  if (lane == 0) {
-    l.waves[0][wave] = above;
-    l.waves[1][wave] = in_bin;
-  }
-  __syncthreads();
-  int at = 0, all_above = 0, all = 0;
-  for (int k = 0; k < kHeavyWaves; ++k) {
-    if (k < wave) at += l.waves[1][k];
-    all_above += l.waves[0][k];
-    all += l.waves[1][k];
-  }
-  const int64_t slice = b * p.slices + blockIdx.x;
-  if (threadIdx.x == 0) p.listed[slice] = make_int2(all_above, all);
-  uint32_t* to = p.list + slice * kSlice;
+  int at = f.before;
+  for (int k = 0; k < wave; ++k) at += l.waves[1][k];
+  uint32_t* to = p.list + b * p.slices * kSlice;
 #pragma unroll
   for (int i = 0; i < kHold; ++i) {
     const uint32_t u = order_of(v[i]);
-    const bool in = held_at(from, i) < s.last && u >> 21 == digit;
+    const bool in = held_at(from, i) < s.last && u >> 21 == f.digit;
     const uint64_t which = __ballot(in);
     if (in) to[at + __popcll(which & (((uint64_t)1 << lane) - 1))] = u;
     at += __popcll(which);
@@ -365,44 +371,39 @@ __global__ __launch_bounds__(kHeavyThreads) void heaviest_write_kernel(const Hea
   __shared__ HeavyLds l;
   __shared__ int sums[2];
   const int64_t b = blockIdx.y;
-  const int tid = (int)threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int tid = (int)threadIdx.x, lane = tid % kWave;
   const HeavySpan s = heavy_span(p, b);
   const int from = s.first + (int)blockIdx.x * kSlice;
   if (s.need <= 0 || from >= s.last) return;
   float v[kHold];
   hold(p.weights + b * p.stride, from, s.last, v);
-  const int used = (s.last - s.first + kSlice - 1) / kSlice;
-  const int2* listed = p.listed + b * p.slices;
+  clear_bins(l);
   int need = s.need;
-  uint32_t bound = first_digit(l, p, b, s, need) << 21, mask = 2047u << 21;
-  // a wave a slice's list, and more of them where it is long
-  auto each = [&](int slices, auto f) {
-    for (int k = 0; k < slices; ++k) {
-      const uint32_t* list = p.list + (b * p.slices + k) * kSlice;
-      const int n = listed[k].y;
-      for (int i = (tid + (k * 2 + 1) * (kHeavyThreads / 2)) % kHeavyThreads; i < n; i += kHeavyThreads) f(list[i]);
-    }
-  };
+  const FirstDigit f = first_digit(l, p, b, s, need);
+  uint32_t bound = f.digit << 21, mask = 2047u << 21;
+  const uint32_t* list = p.list + b * p.slices * kSlice;
 #pragma unroll
   for (int round = 1; round < 3; ++round) {
     const int shift = round == 1 ? 10 : 0;
     const uint32_t digits = round == 2 ? 1023u : 2047u;
-    clear_bins<kCopies>(l);
-    each(used, [&](uint32_t u) {
-      if ((u & mask) == bound) atomicAdd(&l.hist[wave % kCopies][u >> shift & digits], 1);
-    });
-    bound |= (uint32_t)pick_bin<kCopies>(l, need) << shift;
+#pragma unroll 4
+    for (int i = tid; i < f.all; i += kHeavyThreads) {
+      const uint32_t u = list[i];
+      if ((u & mask) == bound) add_to_bin(l, round, u >> shift & digits);
+    }
+    bound |= (uint32_t)pick_bin(l, round, need) << shift;
     mask |= digits << shift;
   }
   // what stays of the slices before this one
   if (tid < 2) sums[tid] = 0;
   __syncthreads();
   int above = 0, same = 0;
-  each((int)blockIdx.x, [&](uint32_t u) {
+#pragma unroll 4
+  for (int i = tid; i < f.before; i += kHeavyThreads) {
+    const uint32_t u = list[i];
     above += u > bound;
     same += u == bound;
-  });
-  for (int k = tid; k < (int)blockIdx.x; k += kHeavyThreads) above += listed[k].x;
+  }
 #pragma unroll
   for (int o = 1; o < kWave; o <<= 1) {
     above += __shfl_xor(above, o);
@@ -413,7 +414,7 @@ __global__ __launch_bounds__(kHeavyThreads) void heaviest_write_kernel(const Hea
     atomicAdd(&sums[1], same);
   }
   __syncthreads();
-  write_kept(l, p, b, v, from, s.last, bound, need, sums[1], p.sinks + sums[0] + min(need, sums[1]));
+  write_kept(l, p, b, v, from, s.last, bound, need, sums[1], p.sinks + f.above + sums[0] + min(need, sums[1]));
 }
 
 int heavy_slices(int64_t positions) { return (int)ceil_div(positions > 0 ? positions : 1, kSlice); }
@@ -566,7 +567,7 @@ extern "C" int fcmoe_draft_tree(const int32_t* parents, int64_t tokens, const in
 extern "C" size_t fcmoe_heaviest_positions_workspace_bytes(int64_t batch, int64_t positions, int64_t keep, int64_t sinks, int64_t recent) {
   if (check_heavy(batch, positions, 0, keep, sinks, recent) != FCMOE_OK || batch == 0) return 0;
   const int64_t slices = heavy_slices(positions);
-  return slices == 1 ? 0 : heavy_list_bytes(batch, slices) + heavy_hist_bytes(batch, slices) + (size_t)batch * (size_t)slices * 8;
+  return slices == 1 ? 0 : heavy_list_bytes(batch, slices) + heavy_hist_bytes(batch, slices);
 }
 
 extern "C" int fcmoe_heaviest_positions(const float* weights, int64_t batch, int64_t positions, int64_t stride,
@@ -590,7 +591,6 @@ extern "C" int fcmoe_heaviest_positions(const float* weights, int64_t batch, int
   if ((uintptr_t)workspace % 16) return fail(FCMOE_EINVAL, "heaviest_positions: unaligned workspace");
   p.list = (uint32_t*)workspace;
   p.hist = (int*)((char*)workspace + heavy_list_bytes(batch, p.slices));
-  p.listed = (int2*)((char*)p.hist + heavy_hist_bytes(batch, p.slices));
   const dim3 g((unsigned)p.slices, (unsigned)batch), t(kHeavyThreads);
   hipLaunchKernelGGL(heaviest_count_kernel, g, t, 0, stream, p);
   hipLaunchKernelGGL(heaviest_list_kernel, g, t, 0, stream, p);
