@@ -324,15 +324,24 @@ struct Stager {
   static __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(uint64_t base, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)bytes, kBufWord3);
   }
-  // Its key parts and scales on their way to registers.
+  // Its key parts and scales on their way to registers. (A shuffle keeps the lane's number in a register from the
+  // kernel's start; FORMED: none to spare.)
+  template <bool FORMED = false>
   __device__ __forceinline__ void parts(const Absorbed& p) {
     if constexpr (P > 0) {
       const uint32_t ln = (uint32_t)lane_now();
       const uint64_t rope = (uint64_t)p.c.rope + (id * p.c.rope_page_stride + in * p.c.rope_row_stride) * T::ELEM;
 #pragma unroll
-      for (int u = 0; u < T::RLOADS; ++u)
-        part[u] = *(const global_v4i*)(__shfl((unsigned long long)rope, u * (64 / T::RUNITS) + (int)(ln / T::RUNITS)) +
-                                       (ln % T::RUNITS) * 16);
+      for (int u = 0; u < T::RLOADS; ++u) {
+        const int from = u * (64 / T::RUNITS) + (int)(ln / T::RUNITS);
+        uint64_t row;
+        if constexpr (FORMED)
+          row = (uint64_t)(uint32_t)__builtin_amdgcn_ds_bpermute(4 * from, (int)(rope >> 32)) << 32 |
+                (uint32_t)__builtin_amdgcn_ds_bpermute(4 * from, (int)(uint32_t)rope);
+        else
+          row = __shfl((unsigned long long)rope, from);
+        part[u] = *(const global_v4i*)(row + (ln % T::RUNITS) * 16);
+      }
     }
     if constexpr (F8) scale = p.c.scale[id * p.c.scale_page_stride + in];
   }
@@ -1164,8 +1173,9 @@ AbsPlan absorbed_plan(const fcmoe_absorbed_args* a, const fcmoe_key_mask* mask) 
   int dev = 0, cus = 256;
   if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
     (void)hipGetLastError();
-  // One workgroup a CU (two LDS buffers fill it); 8-bit rows of 16 leave room for two.
-  const int64_t slots = pl.rows == 128 ? cus / 2 : (int64_t)cus * (a->cache.e4m3 && pl.rows == 16 ? 2 : 1);
+  // One workgroup a CU (two LDS buffers fill it); 8-bit rows of 16 leave room for two. 128 rows take two workgroups, in
+  // the masked form one.
+  const int64_t slots = pl.rows == 128 && !mask ? cus / 2 : (int64_t)cus * (a->cache.e4m3 && pl.rows == 16 ? 2 : 1);
   int64_t tiles = a->table_width > 0 ? ceil_div(a->table_width * a->cache.page_size, kAbsKeys) : 1;
   if (mask && mask->window) {
     const int64_t reach = mask->window + (mask->tree_masks ? a->tokens : pl.rows) - 1;  // as key_tiles
@@ -1181,6 +1191,9 @@ AbsPlan absorbed_plan(const fcmoe_absorbed_args* a, const fcmoe_key_mask* mask) 
   return pl;
 }
 
+template <int R, int P, bool F8>
+void tall_launch(const Absorbed& p, const AbsPlan& pl, hipStream_t stream);  // fcmoe_absorbed_tall.h
+
 template <int R, int P, bool F8, bool MASKED>
 void absorbed_launch(const Absorbed& p, const AbsPlan& pl, hipStream_t stream) {
   const dim3 g((unsigned)pl.shares), b(256);
@@ -1190,6 +1203,8 @@ void absorbed_launch(const Absorbed& p, const AbsPlan& pl, hipStream_t stream) {
     hipLaunchKernelGGL((absorbed_kernel<R, P, F8, 2, 1, MASKED>), g, b, 0, stream, p);
   else if (pl.rows == 64)
     hipLaunchKernelGGL((absorbed_kernel<R, P, F8, 4, 1, MASKED>), g, b, 0, stream, p);
+  else if constexpr (MASKED)
+    tall_launch<R, P, F8>(p, pl, stream);
   else  // pairs lie 8 workgroups apart: whole blocks of 16
     hipLaunchKernelGGL((absorbed_kernel<R, P, F8, 4, 2, MASKED>), dim3((unsigned)(ceil_div(pl.shares, 8) * 16)), b, 0, stream, p);
 }

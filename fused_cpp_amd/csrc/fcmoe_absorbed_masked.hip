@@ -2,6 +2,7 @@
 // context: a sliding window with the sequence's first tokens, and trees of
 // drafted tokens behind it.
 #include "fcmoe_absorbed_kernel.h"
+#include "fcmoe_absorbed_tall.h"
 
 namespace fcmoe {
 
