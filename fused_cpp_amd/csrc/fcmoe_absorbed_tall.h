@@ -573,6 +573,7 @@ __global__ __launch_bounds__(256, 1) void absorbed_tall_kernel(const Absorbed p)
           constexpr int ks = decltype(ks_)::value, at = tall_share(ks, KS, 16);
           if (more) tall_unroll<tall_share(ks + 1, KS, 16) - at>([&](auto k_) { st.load(next, at + decltype(k_)::value); });
         });
+        asm volatile("s_nop 11" : "+v"(s[0]));  // the branches around may pass what follows here by a register of S
       }
       __builtin_amdgcn_sched_barrier(0);
       if (masked) {
