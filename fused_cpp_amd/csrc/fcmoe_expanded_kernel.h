@@ -87,6 +87,17 @@ __device__ __forceinline__ int expanded_limit(const Expanded& p, const SeqSpan& 
 // p and the first `sinks`. A row block walks the tiles of the first keys that its
 // window leaves out, then those from its first row's window on.
 __device__ __forceinline__ int window_low(int pos, int window) { return pos < window ? 0 : pos - window + 1; }
+// Of 32 keys that lie `off` behind a tile's first one, a bit each: which a row sees whose keys at or before it end at
+// `end` of the tile, and whose first ones end at `head`.
+__device__ __forceinline__ uint32_t window_bits(int end, int head, int window, int off) {
+  auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
+  return below(end - off) & (~below(max(max(end, 0) - window, -32) - off) | below(head - off));
+}
+// The value, or -inf where bit k is not set: two instructions, no condition.
+__device__ __forceinline__ float if_seen(float v, uint32_t bits, int k) {
+  const uint32_t all = (uint32_t)((int)(bits << (31 - k)) >> 31);
+  return __uint_as_float((__float_as_uint(v) & all) | (0xff800000u & ~all));
+}
 struct Walk {
   int head_tiles, skip, tiles;  // tile t of the walk is tile t of the sequence for t < head_tiles, else t + skip
   __device__ __forceinline__ int tile(int t) const { return t < head_tiles ? t : t + skip; }
@@ -251,14 +262,13 @@ __global__ __launch_bounds__(kExpWaves * kWave, 2) void expanded_narrow_kernel(c
           if (32 * hf + 8 * (i / 4) + i % 4 >= lim) s[hf][i] = -INFINITY;
     }
     if (WINDOW && tile * kExpKeys < low_max && (tile + 1) * kExpKeys > min(p.sinks, low_max)) {
-      const int low = my_lim - p.window - tile * kExpKeys - 4 * half, head = p.sinks - tile * kExpKeys - 4 * half;
+      const int end = my_lim - tile * kExpKeys - 4 * half, head = p.sinks - tile * kExpKeys - 4 * half;
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
+      for (int hf = 0; hf < 2; ++hf) {
+        const uint32_t sees = window_bits(end, head, p.window, 32 * hf);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int j = 32 * hf + 8 * (i / 4) + i % 4;
-          s[hf][i] = (j < low) & (j >= head) ? -INFINITY : s[hf][i];
-        }
+        for (int i = 0; i < 16; ++i) s[hf][i] = if_seen(s[hf][i], sees, 8 * (i / 4) + i % 4);
+      }
     }
     float top = s[0][0];
 #pragma unroll
@@ -563,19 +573,18 @@ __global__ __launch_bounds__(kExpWaves * kWave, 1) void expanded_wide_kernel(con
     mfma_done<24>(s);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      // keys before end are at or before the row; of these it sees the last
-      // `window` (j - (end - window) below it as unsigned) and those before head
       const int end = lim[r] - tile * kExpKeys;
-      const uint32_t low = WINDOW ? (uint32_t)end - (uint32_t)p.window : 0;
-      const int head = WINDOW ? min(p.sinks - tile * kExpKeys - 4 * half, end) : 0;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
+        // in the windowed form by bits: a condition for each value is long code (a masked tile took 2600 clocks more, of
+        // 4200), and with branches wrong in what the compiler made of it
+        const uint32_t sees = WINDOW ? window_bits(end, p.sinks - tile * kExpKeys - 4 * half, p.window, 32 * hf) : 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int j = 32 * hf + 8 * (i / 4) + i % 4;
-          if constexpr (WINDOW)  // without a branch: one around each of these values is long code, and wrong in what the compiler made of it
-            s[r][hf][i] = ((uint32_t)j - low < (uint32_t)p.window) | (j < head) ? s[r][hf][i] : -INFINITY;
-          else if (j >= end)
+          const int j = 8 * (i / 4) + i % 4;
+          if constexpr (WINDOW)
+            s[r][hf][i] = if_seen(s[r][hf][i], sees, j);
+          else if (32 * hf + j >= end)
             s[r][hf][i] = -INFINITY;
         }
         whole(s[r][hf]);
