@@ -106,6 +106,7 @@ struct Heavy {
   int slices;    // of a sequence's columns; 1: one launch
   int* hist;       // [batch, slices][kBins], first digits
   uint32_t* list;  // [batch][slices * kSlice], the weights of the chosen bin, in their positions' order
+  struct FirstDigit* first;  // [batch, slices]
 };
 
 __device__ __forceinline__ uint32_t order_of(float w) {
@@ -116,21 +117,28 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 
 // Sum over the lanes before this one, and in *total over all.
 __device__ __forceinline__ int lanes_before(int v, int* total) {
-  int upto = v;
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int u = __shfl_up(upto, o);
-    if ((int)threadIdx.x % kWave >= o) upto += u;
-  }
-  *total = __shfl(upto, kWave - 1);
+  const int upto = (int)wave_scan(v);
+  *total = __builtin_amdgcn_readlane(upto, kWave - 1);
   return upto - v;
 }
 
 struct HeavyLds {
   alignas(16) int hist[kCopies][kBins];
-  int waves[2][kHeavyWaves];
+  alignas(16) int waves[2][kHeavyWaves];
   int found[2];  // digit, how many of its bin
 };
+
+// Sum of the waves' values before this wave's.
+__device__ __forceinline__ int waves_before(const int (&of)[kHeavyWaves]) {
+  const int wave = (int)threadIdx.x / kWave;
+  int sum = 0;
+#pragma unroll
+  for (int v = 0; v < kHeavyWaves; v += 4) {
+    const int4 n = *(const int4*)&of[v];
+    sum += (v < wave ? n.x : 0) + (v + 1 < wave ? n.y : 0) + (v + 2 < wave ? n.z : 0) + (v + 3 < wave ? n.w : 0);
+  }
+  return sum;
+}
 
 __device__ __forceinline__ void clear_bins(HeavyLds& l) {
   for (int k = (int)threadIdx.x; k < kCopies * kBins / 4; k += kHeavyThreads) ((int4*)l.hist[0])[k] = make_int4(0, 0, 0, 0);
@@ -144,7 +152,7 @@ __device__ __forceinline__ int pick_bin(HeavyLds& l, int n0, int n1, int& need) 
   int before = lanes_before(n0 + n1, &total);
   if (lane == 0) l.waves[0][wave] = total;
   __syncthreads();
-  for (int v = 0; v < wave; ++v) before += l.waves[0][v];
+  before += waves_before(l.waves[0]);
   if (before < need && before + n0 + n1 >= need) {
     const bool upper = before + n0 >= need;
     l.found[0] = kBins - 1 - 2 * tid - (upper ? 0 : 1);
@@ -233,11 +241,9 @@ __device__ __forceinline__ void write_kept(HeavyLds& l, const Heavy& p, int64_t 
     l.waves[1][wave] = same;
   }
   __syncthreads();
-  for (int k = 0; k < wave; ++k) {
-    const int s = l.waves[1][k];
-    at += l.waves[0][k] + max(min(need - ties, s), 0);
-    ties += s;
-  }
+  const int ties_before = waves_before(l.waves[1]);
+  at += waves_before(l.waves[0]) + min(need, ties + ties_before) - min(need, ties);
+  ties += ties_before;
   const uint64_t lower = ((uint64_t)1 << lane) - 1;
 #pragma unroll
   for (int i = 0; i < kHold; ++i) {
@@ -310,9 +316,11 @@ __global__ __launch_bounds__(kHeavyThreads) void heaviest_count_kernel(const Hea
 struct FirstDigit {
   uint32_t digit;
   int above, before, all;  // weights above the bin in the slices before this one; in the bin there, in all slices
+  int need;                // of the bin's
 };
-__device__ __forceinline__ FirstDigit first_digit(HeavyLds& l, const Heavy& p, int64_t b, const HeavySpan& s, int& need) {
+__device__ __forceinline__ FirstDigit first_digit(HeavyLds& l, const Heavy& p, int64_t b, const HeavySpan& s) {
   __shared__ int sums[3];
+  int need = s.need;
   const int used = (s.last - s.first + kSlice - 1) / kSlice, lo = kBins - 2 - 2 * (int)threadIdx.x;
   const int* h = p.hist + b * p.slices * kBins + lo;
   int n0 = 0, n1 = 0, m0 = 0, m1 = 0;
@@ -335,7 +343,7 @@ __device__ __forceinline__ FirstDigit first_digit(HeavyLds& l, const Heavy& p, i
   for (int o = 1; o < kWave; o <<= 1) above += __shfl_xor(above, o);
   if ((int)threadIdx.x % kWave == 0 && above) atomicAdd(&sums[0], above);
   __syncthreads();
-  return FirstDigit{(uint32_t)digit, sums[0], sums[1], sums[2]};
+  return FirstDigit{(uint32_t)digit, sums[0], sums[1], sums[2], need};
 }
 
 __global__ __launch_bounds__(kHeavyThreads) void heaviest_list_kernel(const Heavy p) {
@@ -347,15 +355,14 @@ __global__ __launch_bounds__(kHeavyThreads) void heaviest_list_kernel(const Heav
   if (s.need <= 0 || from >= s.last) return;
   float v[kHold];
   hold(p.weights + b * p.stride, from, s.last, v);
-  int need = s.need;
-  const FirstDigit f = first_digit(l, p, b, s, need);
+  const FirstDigit f = first_digit(l, p, b, s);
+  if (threadIdx.x == 0) p.first[b * p.slices + blockIdx.x] = f;
   int in_bin = 0;
 #pragma unroll
   for (int i = 0; i < kHold; ++i) in_bin += __popcll(__ballot(held_at(from, i) < s.last && order_of(v[i]) >> 21 == f.digit));
   if (lane == 0) l.waves[1][wave] = in_bin;
   __syncthreads();
-  int at = f.before;
-  for (int k = 0; k < wave; ++k) at += l.waves[1][k];
+  int at = f.before + waves_before(l.waves[1]);
   uint32_t* to = p.list + b * p.slices * kSlice;
 #pragma unroll
   for (int i = 0; i < kHold; ++i) {
@@ -377,20 +384,29 @@ __global__ __launch_bounds__(kHeavyThreads) void heaviest_write_kernel(const Hea
   if (s.need <= 0 || from >= s.last) return;
   float v[kHold];
   hold(p.weights + b * p.stride, from, s.last, v);
-  clear_bins(l);
-  int need = s.need;
-  const FirstDigit f = first_digit(l, p, b, s, need);
-  uint32_t bound = f.digit << 21, mask = 2047u << 21;
+  const FirstDigit f = p.first[b * p.slices + blockIdx.x];
   const uint32_t* list = p.list + b * p.slices * kSlice;
+  // the list's first kHold a thread stay in registers: most lists have no more
+  uint32_t held[kHold];
+#pragma unroll
+  for (int i = 0; i < kHold; ++i) held[i] = i * kHeavyThreads + tid < f.all ? list[i * kHeavyThreads + tid] : 0;
+  auto each = [&](int end, auto use) {
+#pragma unroll
+    for (int i = 0; i < kHold; ++i)
+      if (i * kHeavyThreads + tid < end) use(held[i]);
+#pragma unroll 4
+    for (int i = kHold * kHeavyThreads + tid; i < end; i += kHeavyThreads) use(list[i]);
+  };
+  clear_bins(l);
+  int need = f.need;
+  uint32_t bound = f.digit << 21, mask = 2047u << 21;
 #pragma unroll
   for (int round = 1; round < 3; ++round) {
     const int shift = round == 1 ? 10 : 0;
     const uint32_t digits = round == 2 ? 1023u : 2047u;
-#pragma unroll 4
-    for (int i = tid; i < f.all; i += kHeavyThreads) {
-      const uint32_t u = list[i];
+    each(f.all, [&](uint32_t u) {
       if ((u & mask) == bound) add_to_bin(l, round, u >> shift & digits);
-    }
+    });
     bound |= (uint32_t)pick_bin(l, round, need) << shift;
     mask |= digits << shift;
   }
@@ -398,12 +414,10 @@ __global__ __launch_bounds__(kHeavyThreads) void heaviest_write_kernel(const Hea
   if (tid < 2) sums[tid] = 0;
   __syncthreads();
   int above = 0, same = 0;
-#pragma unroll 4
-  for (int i = tid; i < f.before; i += kHeavyThreads) {
-    const uint32_t u = list[i];
+  each(f.before, [&](uint32_t u) {
     above += u > bound;
     same += u == bound;
-  }
+  });
 #pragma unroll
   for (int o = 1; o < kWave; o <<= 1) {
     above += __shfl_xor(above, o);
@@ -419,6 +433,7 @@ __global__ __launch_bounds__(kHeavyThreads) void heaviest_write_kernel(const Hea
 
 int heavy_slices(int64_t positions) { return (int)ceil_div(positions > 0 ? positions : 1, kSlice); }
 size_t heavy_list_bytes(int64_t batch, int64_t slices) { return (size_t)batch * (size_t)slices * kSlice * 4; }
+size_t heavy_first_bytes(int64_t batch, int64_t slices) { return (size_t)batch * (size_t)slices * sizeof(FirstDigit); }
 size_t heavy_hist_bytes(int64_t batch, int64_t slices) { return (size_t)batch * (size_t)slices * kBins * 4; }
 
 int check_heavy(int64_t batch, int64_t positions, int64_t stride, int64_t keep, int64_t sinks, int64_t recent) {
@@ -455,10 +470,11 @@ __device__ __forceinline__ int2 cached_at(const Move& p, const int32_t* table, i
   return make_int2(id, (int)(at - page * p.c.page_size));
 }
 
+constexpr int kMoveRows = 32;  // 64 sequences of up to 2048 kept rows: 72.7 us with 16, 63.0 with 32, 65.7 with 64
 // To rows that no row of the call is read from: every 16 bytes on their own.
 template <int R, int P, bool F8>
 __global__ __launch_bounds__(256) void move_apart_kernel(const Move p) {
-  constexpr int ELEM = F8 ? 1 : 2, LU = R * ELEM / 16, UNITS = LU + P * ELEM / 16, ROWS = 16;
+  constexpr int ELEM = F8 ? 1 : 2, LU = R * ELEM / 16, UNITS = LU + P * ELEM / 16, ROWS = kMoveRows;
   __shared__ int2 src[ROWS], dst[ROWS];
   const int64_t b = blockIdx.y;
   const int count = move_count(p, b), k0 = (int)blockIdx.x * ROWS, tid = (int)threadIdx.x;
@@ -541,7 +557,7 @@ __global__ __launch_bounds__(1024) void move_within_kernel(const Move p) {
 template <int R, int P, bool F8>
 void move_launch(const Move& p, hipStream_t stream) {
   if (p.to)
-    hipLaunchKernelGGL((move_apart_kernel<R, P, F8>), dim3((unsigned)ceil_div(p.most, 16), (unsigned)p.batch), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((move_apart_kernel<R, P, F8>), dim3((unsigned)ceil_div(p.most, kMoveRows), (unsigned)p.batch), dim3(256), 0, stream, p);
   else
     hipLaunchKernelGGL((move_within_kernel<R, P, F8>), dim3((unsigned)(R * (F8 ? 1 : 2) / 128 + (P || F8 ? 1 : 0)), (unsigned)p.batch),
                        dim3(1024), 0, stream, p);
@@ -567,7 +583,7 @@ extern "C" int fcmoe_draft_tree(const int32_t* parents, int64_t tokens, const in
 extern "C" size_t fcmoe_heaviest_positions_workspace_bytes(int64_t batch, int64_t positions, int64_t keep, int64_t sinks, int64_t recent) {
   if (check_heavy(batch, positions, 0, keep, sinks, recent) != FCMOE_OK || batch == 0) return 0;
   const int64_t slices = heavy_slices(positions);
-  return slices == 1 ? 0 : heavy_list_bytes(batch, slices) + heavy_hist_bytes(batch, slices);
+  return slices == 1 ? 0 : heavy_list_bytes(batch, slices) + heavy_hist_bytes(batch, slices) + heavy_first_bytes(batch, slices);
 }
 
 extern "C" int fcmoe_heaviest_positions(const float* weights, int64_t batch, int64_t positions, int64_t stride,
@@ -591,6 +607,7 @@ extern "C" int fcmoe_heaviest_positions(const float* weights, int64_t batch, int
   if ((uintptr_t)workspace % 16) return fail(FCMOE_EINVAL, "heaviest_positions: unaligned workspace");
   p.list = (uint32_t*)workspace;
   p.hist = (int*)((char*)workspace + heavy_list_bytes(batch, p.slices));
+  p.first = (FirstDigit*)((char*)p.hist + heavy_hist_bytes(batch, p.slices));
   const dim3 g((unsigned)p.slices, (unsigned)batch), t(kHeavyThreads);
   hipLaunchKernelGGL(heaviest_count_kernel, g, t, 0, stream, p);
   hipLaunchKernelGGL(heaviest_list_kernel, g, t, 0, stream, p);
