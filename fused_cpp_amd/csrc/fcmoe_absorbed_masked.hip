@@ -31,10 +31,12 @@ using namespace fcmoe;
 
 extern "C" size_t fcmoe_absorbed_attention_masked_workspace_bytes(const fcmoe_absorbed_args* a, const fcmoe_key_mask* m) {
   if (check_mask(a, m) != FCMOE_OK || a->tokens == 0) return 0;
-  return absorbed_plan(a, m).bytes;
+  const fcmoe_key_mask mask = bounded(*m);
+  return absorbed_plan(a, &mask).bytes;
 }
 
 extern "C" int fcmoe_absorbed_attention_masked(const fcmoe_absorbed_args* a, const fcmoe_key_mask* m, hipStream_t stream) {
   if (const int rc = check_mask(a, m)) return rc;
-  return absorbed_run<true>(a, m, stream);
+  const fcmoe_key_mask mask = bounded(*m);
+  return absorbed_run<true>(a, &mask, stream);
 }

@@ -5,7 +5,9 @@
 using namespace fcmoe;
 
 extern "C" size_t fcmoe_expanded_attention_masked_workspace_bytes(const fcmoe_expanded_args* a, const fcmoe_key_mask* m) {
-  return expanded_sizes_known(a) && m && m->window >= 0 && m->sinks >= 0 ? expanded_plan(a, m).bytes : 0;
+  if (!expanded_sizes_known(a) || !m || m->window < 0 || m->sinks < 0) return 0;
+  const fcmoe_key_mask mask = bounded(*m);
+  return expanded_plan(a, &mask).bytes;
 }
 
 extern "C" int fcmoe_expanded_attention_masked(const fcmoe_expanded_args* a, const fcmoe_key_mask* m, hipStream_t stream) {
@@ -13,5 +15,6 @@ extern "C" int fcmoe_expanded_attention_masked(const fcmoe_expanded_args* a, con
   if (m->window < 0 || m->sinks < 0) return fail(FCMOE_EINVAL, "expanded_attention_masked: window and sinks must not be negative");
   if (m->tree_masks) return fail(FCMOE_EINVAL, "expanded_attention_masked: trees are read in the absorbed form");
   if (!a->causal) return fail(FCMOE_EINVAL, "expanded_attention_masked: a window needs causal");
-  return expanded_run<true>(a, m, stream);
+  const fcmoe_key_mask mask = bounded(*m);
+  return expanded_run<true>(a, &mask, stream);
 }

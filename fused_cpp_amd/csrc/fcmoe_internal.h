@@ -375,5 +375,11 @@ int small_batch_bf16_launch(const SmallBatchArgs& a, bool w8, bool tail, hipStre
 
 // ---- latent attention (fcmoe_latent_rows.hip) ----
 int check_latent_cache(const fcmoe_latent_cache& c, const char* what);
+// Windows and first tokens past 32 bits are past any context; so bounded, their sums stay in 64.
+inline fcmoe_key_mask bounded(fcmoe_key_mask m) {
+  if (m.window > INT32_MAX) m.window = INT32_MAX;
+  if (m.sinks > INT32_MAX) m.sinks = INT32_MAX;
+  return m;
+}
 
 }  // namespace fcmoe

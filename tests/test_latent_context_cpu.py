@@ -255,6 +255,17 @@ def test_cabi_masked_refusals():
     _err(L.fcmoe_expanded_attention_masked(e, cabi.KeyMask(window=9000), None), -2, b"workspace")
 
 
+def test_cabi_windows_past_32_bits_plan_as_ones_past_the_context():
+    L = cabi.lib()
+    b = cabi.AbsorbedArgs(tokens=2, heads=16, batch=2, scale=1.0, cache=_desc(), table_width=1 << 12)
+    e = cabi.ExpandedArgs(tokens=1, keys=100000, heads=1, batch=1, nope_dim=128, v_dim=128, rope_dim=64, scale=1.0, causal=1)
+    wide = cabi.KeyMask(window=1 << 30, sinks=1 << 30)
+    for window, sinks in ((1 << 62, 1 << 62), ((1 << 63) - 1, 0), ((1 << 63) - 1, (1 << 63) - 1), (5, (1 << 63) - 1)):
+        m = cabi.KeyMask(window=window, sinks=sinks)
+        for fn, args in ((L.fcmoe_absorbed_attention_masked_workspace_bytes, b), (L.fcmoe_expanded_attention_masked_workspace_bytes, e)):
+            assert fn(args, m) == fn(args, wide) > 0, (window, sinks)
+
+
 def test_cabi_refusals():
     L = cabi.lib()
     for fn in ("attention_weights", "latent_cache_move"):
