@@ -120,6 +120,7 @@ __global__ __launch_bounds__(kWtWaves* kWave, KT == 1 ? 4 : 2) void weights_kern
     // parts straight from memory, the key parts (rows too short for a load
     // each) through a register
     v4i held{};
+    float held_lse = 0.0f;
     auto take = [&](int chunk, int buf) {
       const int ln = lane_now();
       auto row_of = [&](int at, int& i, int& h) {
@@ -142,6 +143,11 @@ __global__ __launch_bounds__(kWtWaves* kWave, KT == 1 ? 4 : 2) void weights_kern
           held = *(const v4i*)(p.qr + (seq.q0 + i) * p.qrt + h * p.qrh + ln % 8 * 8);
         }
       }
+      const int tid = kWave * wave + ln;
+      if (tid < CH) {
+        row_of(tid, i, h);
+        held_lse = p.lse[(seq.q0 + i) * p.heads + h];
+      }
     };
     auto place = [&](int chunk, int buf) {
       const int ln = lane_now();
@@ -152,10 +158,9 @@ __global__ __launch_bounds__(kWtWaves* kWave, KT == 1 ? 4 : 2) void weights_kern
       }
       const int tid = kWave * wave + ln;
       if (tid < CH) {
-        const int row = chunk * CH + tid, i = min(row, rows - 1) / p.heads, h = min(row, rows - 1) - i * p.heads;
-        const float l = p.lse[(seq.q0 + i) * p.heads + h];
+        const int row = chunk * CH + tid, i = min(row, rows - 1) / p.heads;
         const int v = seq.len - seq.n + i + 1;
-        info[buf][tid] = make_float2(row >= rows || l == -INFINITY ? INFINITY : l * kLog2e, __int_as_float(v < 0 ? 0 : v));
+        info[buf][tid] = make_float2(row >= rows || held_lse == -INFINITY ? INFINITY : held_lse * kLog2e, __int_as_float(v < 0 ? 0 : v));
       }
     };
 
@@ -212,14 +217,25 @@ __global__ __launch_bounds__(kWtWaves* kWave, KT == 1 ? 4 : 2) void weights_kern
       for (int r = 0; r < MT; ++r)
 #pragma unroll
         for (int t = 0; t < KT; ++t) s[r][t] = v4f{0, 0, 0, 0};
+      // Query fragments are read AHEAD uses ahead, in a pinned order: left to itself the compiler reads each where it is used,
+      // and every one waits out the LDS latency.
+      constexpr int READS = KS * MT, AHEAD = KT == 1 ? 1 : 4, RING = AHEAD + 1;
+      v8bf q[RING];
+      auto read = [&](int n) {
+        const int ks = n / MT, r = n % MT;
+        q[n % RING] = *(const __attribute__((address_space(3))) v8bf*)(base + q_at(ks) + 16 * r * (ks < RS ? 2 * R : 2 * P));
+      };
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+      for (int n = 0; n < AHEAD; ++n) read(n);
 #pragma unroll
-        for (int r = 0; r < MT; ++r) {
-          const v8bf q = *(const __attribute__((address_space(3))) v8bf*)(base + q_at(ks) + 16 * r * (ks < RS ? 2 * R : 2 * P));
+      for (int n = 0; n < READS; ++n) {
+        if (n + AHEAD < READS) read(n + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int t = 0; t < KT; ++t) s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][ks], q, s[r][t], 0, 0, 0);
-        }
+        for (int t = 0; t < KT; ++t)
+          s[n % MT][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][n / MT], q[n % RING], s[n % MT][t], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int r = 0; r < MT; ++r) {
         const float2 in = info[buf][16 * r + cr];
