@@ -19,6 +19,10 @@
 // The blocks of 128 KT keys of all sequences are divided evenly among the
 // workgroups. Where a sequence has many rows they are split too (`splits`), each
 // split's sums left in the workspace for a second launch to add in order.
+//
+// 64 sequences of up to 8192, 16 heads 69 us, 4.5 TB/s; 32 tokens of 128 heads
+// over 2 x 16384 170 us, 0.9 PFLOP/s (188 with each query fragment read where it
+// is used and lse between the chunks).
 #include "fcmoe_internal.h"
 #include "fcmoe_latent.h"
 
