@@ -1156,7 +1156,7 @@ __global__ __launch_bounds__(256) void absorbed_combine_kernel(const Absorbed p)
 // ---- host ---------------------------------------------------------------------------
 
 struct AbsPlan {
-  int rows;        // of a row group: 16, 32, 64, or 128 in two workgroups
+  int rows;        // of a row group: 16, 32, 64, or 128 in two workgroups (masked: one)
   int64_t groups;  // upper bound of the batch's row groups
   int64_t shares;  // the units are divided into
   bool by_group;
