@@ -102,9 +102,10 @@ __device__ __forceinline__ int row_groups(const Absorbed& p, const SeqSpan& s, i
 // window + 1 .. p and the first `sinks` tokens; a drafted node, whose position
 // is the context's length plus its depth, the context so and of the nodes
 // those whose bits its mask has. So the rows of a group see no keys but 0 ..
-// head - 1 and lo .. hi - 1: only tiles with some of those are walked, and a
-// tile's other keys are read as a copy of key lo (their pages may be gone; the
-// scores are masked).
+// head - 1 and lo .. hi - 1 (of a tree the context from what depth 0 sees on
+// and the nodes that a mask has bits for): only tiles with some of those are
+// walked, and a tile's other keys are read as a copy of key lo or hi - 1 (their
+// pages may be gone; the scores are masked).
 __device__ __forceinline__ int window_low(int pos, int window) { return pos < window ? 0 : pos - window + 1; }
 struct Seen {
   int head, lo, hi;
@@ -115,7 +116,7 @@ struct Seen {
 __device__ __forceinline__ Seen seen_by(const Absorbed& p, const SeqSpan& s, int i0, int i1) {
   const int base = s.len - s.n;
   Seen v;
-  v.hi = p.tree ? s.len : min(max(base + i1 + 1, 0), s.len);
+  v.hi = p.tree ? max(base + min(s.n, 32 * p.tree_words), 0) : min(max(base + i1 + 1, 0), s.len);
   v.lo = window_low(p.tree ? base : base + i0, p.window);
   v.head = min(p.sinks, v.lo);
   v.head_tiles = (v.head + kAbsKeys - 1) / kAbsKeys;
