@@ -125,6 +125,9 @@ __device__ __forceinline__ Seen seen_by(const Absorbed& p, const SeqSpan& s, int
   return v;
 }
 
+// Depths count as the nearest of 0 .. n - 1, which is all that the walk and the choice of masked tiles reckon with.
+__device__ __forceinline__ int node_depth(const SeqSpan& s, int depth) { return min(max(depth, 0), s.n - 1); }
+
 // Tiles of a row group; at least one, so that a sequence without keys still gets its rows written. The masked form's
 // groups hold different tokens where a sequence has several and no tree: the most that one of them can walk.
 template <bool MASKED>
@@ -817,7 +820,7 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
                 const uint32_t hi = *(const __attribute__((address_space(3))) uint32_t*)(w + 4);
                 bits = off < 0 ? lo << -off : __builtin_amdgcn_alignbit(hi, lo, off);
               }
-              pos = *(lds_i32*)(lds + DEPTH + (16 * r + ml % 16) * 4);
+              pos = node_depth(seq, *(lds_i32*)(lds + DEPTH + (16 * r + ml % 16) * 4));
               up = base;
             } else {
               up = absorbed_limit(seq, pos);

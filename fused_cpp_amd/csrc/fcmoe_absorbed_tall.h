@@ -445,7 +445,7 @@ __global__ __launch_bounds__(256, 1) void absorbed_tall_kernel(const Absorbed p)
             const uint32_t hi = *(const __attribute__((address_space(3))) uint32_t*)(w + 4);
             bits = off < 0 ? lo << -off : __builtin_amdgcn_alignbit(hi, lo, off);
           }
-          pos = *(lds_i32*)(lds + DEPTH + (32 * wave + ml % 32) * 4);
+          pos = node_depth(seq, *(lds_i32*)(lds + DEPTH + (32 * wave + ml % 32) * 4));
           up = base;
         } else {
           up = absorbed_limit(seq, pos);

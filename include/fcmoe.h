@@ -336,8 +336,9 @@ int fcmoe_absorbed_attention(const fcmoe_absorbed_args* args, hipStream_t stream
  * nodes past the mask's words are not seen. No cached row outside what some row
  * sees is read, but for copies of ones that are: its pages may be gone. With a
  * tree that is the context from what a node of depth 0 sees on, and all nodes
- * that the mask's words have bits for, whether set or not. Masks have 1 to 16
- * words a token, rows mask_stride words apart. */
+ * that the mask's words have bits for, whether set or not. Depths count as the
+ * nearest of 0 .. n - 1. Masks have 1 to 16 words a token, rows mask_stride
+ * words apart. */
 typedef struct fcmoe_key_mask {
   int64_t window, sinks;
   const uint64_t* tree_masks; /* [tokens, mask_words] or NULL */

@@ -1,8 +1,10 @@
-"""GPU trees of drafts whose cache holds less than the sequences' lengths say: nodes that no mask has a bit for."""
+"""GPU trees of drafts at the ends of what their masks and depths say: nodes that no mask has a bit for, and depths that no
+tree of the call's nodes has."""
 
 from __future__ import annotations
 
 import pytest
+import torch
 
 from tests import context_reference as cref
 from tests import latent_reference as ref
@@ -35,5 +37,30 @@ def test_nodes_past_the_masks_may_be_gone(gpu, H, singles, dtype, window, sinks)
     _forget(pg, lens, keeps)
     out, lse = la.absorbed_attention(ql, qr, pg.cache, pg.table, pg.lens, scale=0.07, query_starts=st, tree=tree, window=window,
                                      sinks=sinks, return_lse=True)
+    ref.assert_within(out, want, tol, "out")
+    ref.assert_within(lse, wl, ltol, "lse")
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("H", [1, 4, 6, 12, 16, 128])
+def test_depths_count_as_ones_of_the_nodes(gpu, H, dtype):
+    """Depths of a user's own below 0 count as 0, ones past the last node's number as that. (Row groups of 16, 32, 64, 128.)"""
+    la, lc = _la(), _lc()
+    given = [[0, -1, 3, 2 ** 31 - 1], [-2 ** 31, 200, 1], [70], [-7, 9, 5, 4, 3, 2, 1, 0, 100]]
+    context, (window, sinks) = [400, 130, 65, 200], (70, 3)
+    new = [len(d) for d in given]
+    lens = [c + n for c, n in zip(context, new)]
+    pg = _Paged(H, lens, 512, 64, dtype, page=16)
+    st = _i32(_starts(new))
+    ql, qr = _queries(4, sum(new), H, 512, 64)
+    masks = torch.tensor([[1 << i] for n in new for i in range(n)], dtype=torch.int64, device="cuda")
+    keeps = []
+    for c, d in zip(context, given):
+        n, j = len(d), torch.arange(c + len(d), device="cuda")
+        at = torch.tensor([c + min(max(v, 0), n - 1) for v in d], device="cuda")[:, None]
+        keeps.append(((j < c) & ((j > at - window) | (j < sinks))) | (j == c + torch.arange(n, device="cuda")[:, None]))
+    want, wl, tol, ltol = cref.absorbed(ql, qr, pg.rows, _starts(new), 0.07, keeps)
+    out, lse = la.absorbed_attention(ql, qr, pg.cache, pg.table, pg.lens, scale=0.07, query_starts=st, window=window, sinks=sinks,
+                                     tree=lc.DraftTree(masks, _i32([v for d in given for v in d])), return_lse=True)
     ref.assert_within(out, want, tol, "out")
     ref.assert_within(lse, wl, ltol, "lse")
