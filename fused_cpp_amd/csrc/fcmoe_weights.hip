@@ -83,7 +83,7 @@ __global__ __launch_bounds__(kWtWaves* kWave, KT == 1 ? 4 : 2) void weights_kern
   constexpr int MT = CH / 16, CHUNK = CH * 2 * (R + P);
   constexpr int BLOCK = kWtWaves * 16 * KT;
   __shared__ __align__(1024) uint8_t smem[2 * CHUNK];
-  __shared__ float2 info[2][CH];  // a row's log2 of its sum (inf: no weights), and the keys it sees as an integer
+  __shared__ float2 info[2][CH];  // a row's log2 of its sum, and the keys it sees as an integer (0: it has no weights)
   lds_u8* lds = (lds_u8*)smem;
   const int lane = (int)threadIdx.x % kWave, wave = wave_index();
   const int lq = lane / 16, lr = lane % 16;
@@ -162,9 +162,10 @@ __global__ __launch_bounds__(kWtWaves* kWave, KT == 1 ? 4 : 2) void weights_kern
       }
       const int tid = kWave * wave + ln;
       if (tid < CH) {
+        // a place without a row, or a row without a sum, sees no keys: its scores may then be anything, NaN as well
         const int row = chunk * CH + tid, i = min(row, rows - 1) / p.heads;
-        const int v = seq.len - seq.n + i + 1;
-        info[buf][tid] = make_float2(row >= rows || held_lse == -INFINITY ? INFINITY : held_lse * kLog2e, __int_as_float(v < 0 ? 0 : v));
+        const bool counts = row < rows && held_lse != -INFINITY;
+        info[buf][tid] = make_float2(counts ? held_lse * kLog2e : 0.0f, __int_as_float(counts ? max(seq.len - seq.n + i + 1, 0) : 0));
       }
     };
 

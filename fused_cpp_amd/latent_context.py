@@ -51,10 +51,11 @@ def attention_weights(q_latent: torch.Tensor, q_rope: Optional[torch.Tensor], ca
     ``previous``: ``[B, positions]`` fp32 by position in the sequence.
 
     The queries, cache and lengths of a causal :func:`~fused_cpp_amd.latent_attention.absorbed_attention` and the
-    ``lse`` that it returned. Positions are ``previous``'s (or ``out``'s) columns, else the page table's reach; tokens past them are left out, and places
-    past a length keep what they had (0 without ``previous``). ``out`` may be ``previous`` itself. A query whose lse
-    is -inf adds nothing; a page id outside the cache makes its tokens' weights NaN. Sums are taken in fp32, in an
-    order that only the shapes and lengths decide.
+    ``lse`` that it returned. Positions are ``previous``'s (or ``out``'s) columns, else the page table's reach; tokens
+    past them are left out, and places past a length keep what they had (0 without ``previous``). ``out`` may be
+    ``previous`` itself. A query whose lse is -inf adds nothing, whatever its row holds; a page id outside the cache makes
+    the weights of its tokens that other queries see NaN. Sums are taken in fp32, in an order that only the shapes and
+    lengths decide.
     """
     return _native.require_native().latent_attention_weights(
         q_latent, q_rope, cache.latent, cache.rope, cache.scale, page_table, kv_lens, lse, scale, query_starts,

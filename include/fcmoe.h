@@ -400,8 +400,9 @@ int fcmoe_draft_tree(const int32_t* parents, int64_t tokens, const int32_t* quer
  * fcmoe_absorbed_attention, whose lse [tokens, heads] is given) and their
  * heads; for j < kv_lens[b], else previous[b, j]. out and previous (NULL: zeros) [batch,
  * positions], rows out_stride and previous_stride values apart; out may be
- * previous itself. Rows with an lse of -inf add nothing; a page id outside the
- * cache makes its tokens' weights NaN. batch at most 65535. */
+ * previous itself. Rows with an lse of -inf add nothing, whatever they hold; a
+ * page id outside the cache makes the weights of its tokens that other rows see
+ * NaN. batch at most 65535. */
 typedef struct fcmoe_attention_weights_args {
   const uint16_t* q_latent;
   const uint16_t* q_rope;
