@@ -190,6 +190,13 @@ __device__ __forceinline__ HeavySpan heavy_span(const Heavy& p, int64_t b) {
   return s;
 }
 
+// This workgroup's slice of the compared weights begins here; -1: it has none. (First tokens and columns together may pass
+// 32 bits: the grid covers all columns, whatever the first tokens leave of them.)
+__device__ __forceinline__ int slice_begin(const HeavySpan& s) {
+  const int64_t at = s.first + (int64_t)blockIdx.x * kSlice;
+  return s.need > 0 && at < s.last ? (int)at : -1;
+}
+
 // Weight i of this thread among the slice from position `from` on: a wave has 64 kHold neighbours, 64 of them at a time.
 __device__ __forceinline__ int held_at(int from, int i) {
   return from + ((int)threadIdx.x / kWave * kHold + i) * kWave + (int)threadIdx.x % kWave;
@@ -293,9 +300,9 @@ __global__ __launch_bounds__(kHeavyThreads) void heaviest_count_kernel(const Hea
   __shared__ HeavyLds l;
   const int64_t b = blockIdx.y;
   const HeavySpan s = heavy_span(p, b);
-  const int from = s.first + (int)blockIdx.x * kSlice;
+  const int from = slice_begin(s);
   if (blockIdx.x == 0) write_ends(p, b, s);
-  if (s.need <= 0 || from >= s.last) return;
+  if (from < 0) return;
   float v[kHold];
   hold(p.weights + b * p.stride, from, s.last, v);
   clear_bins(l);
@@ -351,8 +358,8 @@ __global__ __launch_bounds__(kHeavyThreads) void heaviest_list_kernel(const Heav
   const int64_t b = blockIdx.y;
   const int lane = (int)threadIdx.x % kWave, wave = (int)threadIdx.x / kWave;
   const HeavySpan s = heavy_span(p, b);
-  const int from = s.first + (int)blockIdx.x * kSlice;
-  if (s.need <= 0 || from >= s.last) return;
+  const int from = slice_begin(s);
+  if (from < 0) return;
   float v[kHold];
   hold(p.weights + b * p.stride, from, s.last, v);
   const FirstDigit f = first_digit(l, p, b, s);
@@ -380,8 +387,8 @@ __global__ __launch_bounds__(kHeavyThreads) void heaviest_write_kernel(const Hea
   const int64_t b = blockIdx.y;
   const int tid = (int)threadIdx.x, lane = tid % kWave;
   const HeavySpan s = heavy_span(p, b);
-  const int from = s.first + (int)blockIdx.x * kSlice;
-  if (s.need <= 0 || from >= s.last) return;
+  const int from = slice_begin(s);
+  if (from < 0) return;
   float v[kHold];
   hold(p.weights + b * p.stride, from, s.last, v);
   const FirstDigit f = p.first[b * p.slices + blockIdx.x];
