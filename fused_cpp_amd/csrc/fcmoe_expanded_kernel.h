@@ -576,8 +576,10 @@ __global__ __launch_bounds__(kExpWaves * kWave, 1) void expanded_wide_kernel(con
       const int end = lim[r] - tile * kExpKeys;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        // in the windowed form by bits: a condition for each value is long code (a masked tile took 2600 clocks more, of
-        // 4200), and with branches wrong in what the compiler made of it
+        // In the windowed form by bits: a condition for each value is long code (a masked tile took 2600 clocks more, of
+        // 4200). And not by branches: the block that replaces a value under `a || b` is reached by two of them, and the
+        // compiler forms the changed vector ahead of the first only, so that lanes which come by the second keep the
+        // old value. (The plain form's one condition becomes a select.)
         const uint32_t sees = WINDOW ? window_bits(end, p.sinks - tile * kExpKeys - 4 * half, p.window, 32 * hf) : 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
