@@ -14,7 +14,8 @@
     attention_weights(q_latent, q_rope, cache, page_table, kv_lens, lse, scale=..., previous=weights, out=weights)
     positions, kept, kept_weights = heaviest_positions(weights, kv_lens, keep, sinks=4, recent=128)
     latent_cache_move(cache, page_table, positions, kept)    # kept: the new kv_lens
-    weights.zero_()[:, :keep] = kept_weights
+    n = min(keep, weights.shape[1])
+    weights.zero_()[:, :n] = kept_weights[:, :n]             # the rows' sums move with them
 
 Scores, weights and their sums are fp32. Streams, capture into HIP graphs, errors,
 and what written tensors may share are ``latent_attention``'s; inputs that require a
