@@ -564,34 +564,31 @@ __global__ __launch_bounds__(kExpWaves * kWave, 1) void expanded_wide_kernel(con
       between(j_);
     });
   };
-  auto masked = [&](int t) {  // whether some row does not see all of tile t of the walk
+  auto masked = [&](int t) {  // the windowed form's: whether some row does not see all of tile t of the walk
     const int first = walk.tile(t) * kExpKeys, behind = first + kExpKeys;
-    return behind > lim_min || (WINDOW && first < low_max && behind > p.sinks);
+    return behind > lim_min || (first < low_max && behind > p.sinks);
   };
   auto mask = [&](int t) {
-    const int tile = walk.tile(t);
     mfma_done<24>(s);
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int end = lim[r] - tile * kExpKeys;
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        // In the windowed form by bits: a condition for each value is long code (a masked tile took 2600 clocks more, of
-        // 4200). And not by branches: the block that replaces a value under `a || b` is reached by two of them, and the
-        // compiler forms the changed vector ahead of the first only, so that lanes which come by the second keep the
-        // old value. (The plain form's one condition becomes a select.)
-        const uint32_t sees = WINDOW ? window_bits(end, p.sinks - tile * kExpKeys - 4 * half, p.window, 32 * hf) : 0;
+        if constexpr (WINDOW) {
+          // By bits: a condition for each value is long code (a masked tile took 2600 clocks more, of 4200). And not by
+          // branches: the block that replaces a value under `a || b` is reached by two of them, and the compiler forms the
+          // changed vector ahead of the first only, so that lanes which come by the second keep the old value.
+          const int first = walk.tile(t) * kExpKeys;
+          const uint32_t sees = window_bits(lim[r] - first, p.sinks - first - 4 * half, p.window, 32 * hf);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int j = 8 * (i / 4) + i % 4;
-          if constexpr (WINDOW)
-            s[r][hf][i] = if_seen(s[r][hf][i], sees, j);
-          else if (32 * hf + j >= end)
-            s[r][hf][i] = -INFINITY;
+          for (int i = 0; i < 16; ++i) s[r][hf][i] = if_seen(s[r][hf][i], sees, 8 * (i / 4) + i % 4);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)  // one condition, which becomes a select
+            if (32 * hf + 8 * (i / 4) + i % 4 >= lim[r] - t * kExpKeys) s[r][hf][i] = -INFINITY;
         }
         whole(s[r][hf]);
       }
-    }
   };
   // From S to the exponents x, in 16 operations of four.
   auto exponents = [&](int g) {
@@ -609,7 +606,7 @@ __global__ __launch_bounds__(kExpWaves * kWave, 1) void expanded_wide_kernel(con
     for (int ks = 0; ks < kAhead; ++ks) k_read(lds, ks);
     operands_ready();
     scores(lds, [](auto) {});
-    if (masked(t_begin)) mask(t_begin);
+    if (WINDOW ? masked(t_begin) : (t_begin + 1) * kExpKeys > lim_min) mask(t_begin);
     mfma_done<24>(s);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -736,7 +733,7 @@ __global__ __launch_bounds__(kExpWaves * kWave, 1) void expanded_wide_kernel(con
     }
     l[0] += sum[0][0] + sum[0][1];
     l[1] += sum[1][0] + sum[1][1];
-    if (t + 1 < w_end && masked(t + 1)) mask(t + 1);
+    if (t + 1 < w_end && (WINDOW ? masked(t + 1) : (t + 2) * kExpKeys > lim_min)) mask(t + 1);
     unroll<2 * NV>([&](auto j_) {
       constexpr int j = decltype(j_)::value, n = j / 2, r = j % 2;
       if constexpr (r == 0 && n + vAhead < NV) v_read(n + vAhead);
