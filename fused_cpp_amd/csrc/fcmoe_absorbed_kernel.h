@@ -830,7 +830,7 @@ __global__ __launch_bounds__(256, MT == 1 && F8 ? 2 : 1) void absorbed_kernel(co
             for (int i = 0; i < 4; ++i) {
               const int j = j0 + i;
               const bool context = (j < up) & ((j >= low) | (j < b.sinks)), node = (j >= up) & (j < seq.len) & ((bits >> i & 1) != 0);
-              s[r][i] = context | node ? s[r][i] : -INFINITY;
+              s[r][i] = (context | node) ? s[r][i] : -INFINITY;
             }
           }
         }

@@ -477,7 +477,9 @@ __device__ __forceinline__ int2 cached_at(const Move& p, const int32_t* table, i
   return make_int2(id, (int)(at - page * p.c.page_size));
 }
 
-constexpr int kMoveRows = 32;  // 64 sequences of up to 2048 kept rows: 72.7 us with 16, 63.0 with 32, 65.7 with 64
+// Rows of a workgroup, us with 16, 32, 64: 64 sequences of up to 2048 kept rows, rows from memory, 72.7, 63.0, 65.7; of 512 to
+// 2048 53.9, 47.8, 50.2, of 8 bits 28.5, 36.2, 29.3; 16 of 2048 21.4, 18.1, 16.9; 8 of up to 300 4.9, 5.1, 7.5.
+constexpr int kMoveRows = 32;
 // To rows that no row of the call is read from: every 16 bytes on their own.
 template <int R, int P, bool F8>
 __global__ __launch_bounds__(256) void move_apart_kernel(const Move p) {
@@ -520,6 +522,10 @@ __global__ __launch_bounds__(256) void move_apart_kernel(const Move p) {
 // row's place is only ever read for an earlier one (or itself). A workgroup takes
 // 128 bytes of every row of a sequence (the last one the key part and the
 // scales), 1024 rows at a time in order: they are all read before any is written.
+// That is 9 workgroups a sequence (5 of 8-bit rows), each with one chunk's latency
+// behind the other: 1 sequence of 4096 kept rows 48 us (62 of 8 bits), 8 of them 72,
+// 64 of 512 to 2048 99 (68), where the bytes take 2, 16 and 38 (20); up to 5
+// accepted drafts of 32 sequences 4.2.
 template <int R, int P, bool F8>
 __global__ __launch_bounds__(1024) void move_within_kernel(const Move p) {
   constexpr int ELEM = F8 ? 1 : 2, PIECES = R * ELEM / 128, RU = P * ELEM / 16, HOLD = 8;

@@ -388,9 +388,9 @@ int fcmoe_expanded_attention_masked(const fcmoe_expanded_args* args, const fcmoe
 /* Masks and depths of trees of drafted tokens, for fcmoe_key_mask: token i of
  * sequence b (query_starts[b] .. [b + 1]) is a node whose parent is node
  * parents[t] < i of the same sequence; any other value (-1) makes it a root. Bit j
- * of masks [tokens, mask_words] is set for the node itself and its ancestors,
- * depths [tokens] counts those. mask_words 1 to 16: nodes past 64 mask_words
- * of a sequence, and tokens of none, get no bits and depth 0. */
+ * of masks [tokens, mask_words] is set for the node itself and its ancestors;
+ * depths [tokens] counts the ancestors, a root's is 0. mask_words 1 to 16: nodes
+ * past 64 mask_words of a sequence, and tokens of none, get no bits and depth 0. */
 int fcmoe_draft_tree(const int32_t* parents, int64_t tokens, const int32_t* query_starts, int64_t batch, int64_t mask_words,
                      uint64_t* masks, int32_t* depths, hipStream_t stream);
 
