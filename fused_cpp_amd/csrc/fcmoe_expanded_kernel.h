@@ -851,7 +851,7 @@ __global__ __launch_bounds__(kExpWaves * kWave) void expanded_combine_kernel(con
 // Measured wide against narrow, 128 + 64 / 128: 128 heads of 1500
 // tokens 132 us, 129, of 2048 210, 225; 16 heads of 4 x 4096 188, 200; 160 tokens
 // behind 8000, 128 heads, 191, 244; but 32 x 128 tokens, 128 heads, 167, 82.
-// Windows, both ways (rows of equal length): a prompt of 16384, 16 heads, windows of 512 192, 154; 1024 255, 240; 2048 384,
+// Windows, wide and narrow: a prompt of 16384, 16 heads, windows of 512 192, 154; 1024 255, 240; 2048 384,
 // 408; 4096 632, 697; 16 chunks of 256 behind 4000, 32 heads, 1024 154, 143, 2048 228, 246; 5 chunks of up to 333 behind up
 // to 20000, 2048 88, 97. The two meet at some 1500 keys, not at the 1024 that are asked for: a window of 1024 loses 6 to 8%,
 // more with few blocks (512 tokens behind 32000, 16 heads, 37, 27), whose empty places are not counted either.

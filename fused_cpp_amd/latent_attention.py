@@ -164,10 +164,10 @@ def absorbed_attention(q_latent: torch.Tensor, q_rope: Optional[torch.Tensor], c
     pages that hold a token which some query sees are read, so the others may be gone (their table entries anything).
     ``tree`` (of :func:`~fused_cpp_amd.latent_context.draft_tree`, with ``query_starts``): a sequence's n query tokens
     are the nodes of a tree of drafts, cached in their order as its last n tokens. A node sees the ``kv_lens[b] - n``
-    tokens before them and the nodes that its mask has; with a window the ones before them as a token at
-    ``kv_lens[b] - n + depth`` does, and of the nodes still all that its mask has. Depths of a user's own count as the
-    nearest of 0 to n - 1; of the context what a node of depth 0 sees on is read, whatever they are. Nodes past the masks' words are not seen, and neither their rows nor their pages are
-    read; the rows of all others have to be finite.
+    tokens before them and the nodes that its mask has; with a window the ones before them as a token at ``kv_lens[b]
+    - n + depth`` does, and of the nodes still all that its mask has. Depths of a user's own count as the nearest of 0
+    to n - 1; of the context what a node of depth 0 sees on is read, whatever they are. Nodes past the masks' words
+    are not seen, and neither their rows nor their pages are read; the rows of all others have to be finite.
 
     ``return_lse`` adds ``[T, H]`` fp32: the log of the softmax's sum (-inf where there is none), which joins results
     over parts of a context. Tokens that no sequence holds are 0, or left as they were in a given ``out``.
